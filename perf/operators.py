@@ -88,7 +88,8 @@ def _blocks(x, rows):
 def _quantize(x, rows):
     """float32 x in e4m3 with a scale for each block."""
     amax, spread = _blocks(x, rows)
-    return (x * (TOP / spread.clamp(min=LEAST))).to(torch.float8_e4m3fn), amax.clamp(min=LEAST) / TOP
+    top = torch.tensor(TOP, device=x.device)                 # (a quotient with a number would be a product with its reciprocal)
+    return (x * torch.div(top, spread.clamp(min=LEAST))).to(torch.float8_e4m3fn), torch.div(amax.clamp(min=LEAST), top)
 
 
 def _values(q, scales, rows):
