@@ -59,6 +59,12 @@ LIBRARIES: Dict[str, dict] = {
         "flags": [],
         "link": [],
     },
+    "fp8": {
+        "sources": ["quantize_fp8.cu", "gemm_fp8.cu"],
+        "deps": ["mbarrier.cuh", "shared_limit.cuh"],
+        "flags": [],
+        "link": [],
+    },
     # the host library: configuration, weights, parts, cache manager, step function, scheduler, samplers and the C
     # API (api/inference.h); it opens the kernel libraries above by need, from the folder it is loaded from
     "qengine": {

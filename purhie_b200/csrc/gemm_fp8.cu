@@ -1,0 +1,407 @@
+// The matrix product of 8-bit operands with scales, on the 5th-generation tensor cores:
+//
+//   out[m, n] = sum_b xs[m, b] * ws[n / 128, b] * sum_{k in block b} x[m, k] * w[n, k],
+//
+// x [M, K] rows in e4m3 with a float32 scale for each 128 values, w [N, K] a weight in e4m3 with a scale for each block of
+// 128 x 128, both K-major.  The inner sum, over the 128 values that share their scales, is four tcgen05.mma (kind::f8f6f4, 32
+// of K each) into an accumulator in tensor memory that starts from zero; the outer one is float32, in registers: the epilogue
+// warps read each block's accumulator with tcgen05.ld, multiply it by the two scales and add, while the tensor cores work on
+// the next blocks in other accumulators.  A block of K is one stage of the ring: 128 bytes a row, one row of the swizzle.
+//
+// One CTA computes a tile of 128 x BN.  Plain orientation: the 128 rows are tokens, and a thread's scale is its own row's.  Swapped
+// (few tokens): they are features of the weight, which is what has to be streamed, and the tokens lie on the narrow side; the
+// scale then differs by column and comes from shared memory.  Where the tiles are fewer than the CTAs that the device holds, K
+// is cut among the CTAs of a cluster, which leave their sums in shared memory and add them up there, in the order of their
+// ranks: one launch, no workspace, and the same bits every time.
+//
+// Every wait on an mbarrier is bounded; a wait that runs out sets *error_flag, and the CTA still takes part in the cluster's
+// barriers, frees its tensor memory and returns (what it writes is then meaningless).
+// The reference's counterpart is its WMMA tile kernel over 8-bit blocks (src/matvec_q.hip:3437-3547).
+#include "common.cuh"
+#include "mbarrier.cuh"
+#include "shared_limit.cuh"
+
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+
+namespace {
+
+using namespace ph;
+using namespace ph_mbar;
+
+constexpr int BM = 128;
+constexpr int BK = 128;                     // values (bytes) of K in a stage: one block of the scales
+constexpr int UMMA_K = 32;
+constexpr int THREADS = 192;                // copies, products, four epilogue warps
+constexpr int A_BYTES = BM * BK;
+constexpr int SCALE_BLOCKS = 32;            // blocks of K whose scales lie in shared memory at a time (swapped)
+constexpr int MAX_CLUSTER = 8;
+
+#define PH_ERR_FP8_PRODUCER 131
+#define PH_ERR_FP8_MMA 132
+#define PH_ERR_FP8_EPILOGUE 133
+
+struct Params {
+    const float* xs;
+    const float* ws;
+    void* out;
+    int out_bf16;
+    int M, N;
+    int kblocks;
+    int a_tiles, splits;
+    int early_w;
+    int* error_flag;
+};
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c_inner, int c_row) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(smem_addr(bar)), "r"(c_inner), "r"(c_row) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void umma(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+// Shared-memory matrix descriptor of a K-major tile with the 128-byte swizzle: address >> 4 in bits 0-13, groups of eight rows 1024
+// bytes apart (>> 4, bits 32-45), version 1 at bit 46, swizzle mode 2 at bits 61-63.
+__device__ __forceinline__ uint64_t smem_desc(const void* p) {
+    return (uint64_t)((smem_addr(p) & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Instruction descriptor, kind::f8f6f4: D float32 (bits 4-5 = 1), A and B e4m3 (bits 7-9, 10-12 = 0), both K-major, N >> 3 at
+// bits 17-22, M >> 4 at bits 24-28.
+__host__ __device__ constexpr uint32_t make_idesc(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The float at the place of p in the shared memory of the CTA of that rank.
+__device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// Few tokens: two CTAs share an SM, so that one's start and end overlap the other's streaming.
+template <int BN> struct Tile {
+    static constexpr int STAGE_BYTES = A_BYTES + BN * BK;
+    static constexpr int CTAS_PER_SM = BN <= 64 ? 2 : 1;
+    static constexpr int STAGES = (CTAS_PER_SM == 2 ? 96 : 196) * 1024 / STAGE_BYTES;
+    static constexpr int BUFFERS = BN >= 64 ? 4 : 128 / BN;              // accumulators in tensor memory
+    static constexpr int TMEM_COLS = BUFFERS * BN;
+    static constexpr int SUMS_BYTES = BN * (BM + 1) * 4;                 // the tile's sums, in the ring's memory once it is empty
+    static constexpr int SCALES_BYTES = SCALE_BLOCKS * BN * 4;
+    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + SCALES_BYTES + 256;
+    static_assert(SUMS_BYTES <= STAGES * STAGE_BYTES, "the sums do not fit");
+    static_assert(TMEM_COLS * CTAS_PER_SM <= 512, "tensor memory");
+};
+
+template <int BN, bool SWAPPED>
+__global__ void __launch_bounds__(THREADS, Tile<BN>::CTAS_PER_SM)
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, Params p) {
+    using Cfg = Tile<BN>;
+    constexpr int STAGES = Cfg::STAGES, BUFFERS = Cfg::BUFFERS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* smem_a = smem;
+    uint8_t* smem_b = smem + STAGES * A_BYTES;
+    float* sums = (float*)smem;                                          // [BN][BM + 1]
+    float* scales = (float*)(smem + STAGES * Cfg::STAGE_BYTES);          // [SCALE_BLOCKS][BN], swapped
+    uint64_t* full = (uint64_t*)(smem + STAGES * Cfg::STAGE_BYTES + Cfg::SCALES_BYTES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;
+    uint64_t* acc_empty = acc_full + BUFFERS;
+    uint32_t* tmem_slot = (uint32_t*)(acc_empty + BUFFERS);
+    static_assert((2 * STAGES + 2 * BUFFERS) * 8 + 4 <= 256, "barriers");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { init(&full[s], 1); init(&empty[s], 1); }
+        for (int b = 0; b < BUFFERS; ++b) { init(&acc_full[b], 1); init(&acc_empty[b], 4); }
+        fence_init();
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int splits = p.splits, rank = blockIdx.x % splits, tile = blockIdx.x / splits;
+    const int a0 = (tile % p.a_tiles) * BM, b0 = (tile / p.a_tiles) * BN;
+    const int kb0 = (int)((long long)p.kblocks * rank / splits), kb1 = (int)((long long)p.kblocks * (rank + 1) / splits);
+
+    pdl_launch_dependents();
+    float acc[BN];
+    if (warp == 0) {
+        if (lane == 0) {
+            // the weight's tiles of the first stages may not have to wait for the kernel in front
+            int pre = 0;
+            if (p.early_w)
+                for (; pre < STAGES && kb0 + pre < kb1; ++pre) {
+                    arrive_expect_tx(&full[pre], Cfg::STAGE_BYTES);
+                    if (SWAPPED) tma_load_2d(smem_a + pre * A_BYTES, &map_a, &full[pre], (kb0 + pre) * BK, a0);
+                    else tma_load_2d(smem_b + pre * BN * BK, &map_b, &full[pre], (kb0 + pre) * BK, b0);
+                }
+            pdl_wait();
+            for (int s = 0; s < pre; ++s) {
+                if (SWAPPED) tma_load_2d(smem_b + s * BN * BK, &map_b, &full[s], (kb0 + s) * BK, b0);
+                else tma_load_2d(smem_a + s * A_BYTES, &map_a, &full[s], (kb0 + s) * BK, a0);
+            }
+            int stage = pre == STAGES ? 0 : pre;
+            uint32_t phase = pre == STAGES ? 1 : 0;
+            bool ok = true;
+            for (int kb = kb0 + pre; kb < kb1; ++kb) {
+                if (!wait(&empty[stage], phase ^ 1, p.error_flag, PH_ERR_FP8_PRODUCER)) { ok = false; break; }
+                arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
+                tma_load_2d(smem_a + stage * A_BYTES, &map_a, &full[stage], kb * BK, a0);
+                tma_load_2d(smem_b + stage * BN * BK, &map_b, &full[stage], kb * BK, b0);
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+            // not past this point while copies may be in flight: the products have released every stage
+            for (int s = 0; s < STAGES && ok; ++s) {
+                if (!wait(&empty[stage], phase ^ 1, p.error_flag, PH_ERR_FP8_PRODUCER)) break;
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = make_idesc(BM, BN);
+            int stage = 0, buf = 0;
+            uint32_t phase = 0, buf_phase = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!wait(&acc_empty[buf], buf_phase ^ 1, p.error_flag, PH_ERR_FP8_MMA)) break;
+                if (!wait(&full[stage], phase, p.error_flag, PH_ERR_FP8_MMA)) break;
+                tc_fence_after();
+                const uint64_t adesc = smem_desc(smem_a + stage * A_BYTES), bdesc = smem_desc(smem_b + stage * BN * BK);
+#pragma unroll
+                for (int k = 0; k < BK / UMMA_K; ++k)                    // 32 values further along the swizzled row
+                    umma(tmem_base + (uint32_t)(buf * BN), adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k > 0 ? 1u : 0u);
+                umma_commit(&empty[stage]);
+                umma_commit(&acc_full[buf]);
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                if (++buf == BUFFERS) { buf = 0; buf_phase ^= 1; }
+            }
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3;                                          // the quarter of the accumulator's rows that this warp may read
+        const int row = q * 32 + lane;
+        pdl_wait();
+#pragma unroll
+        for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
+        int buf = 0;
+        uint32_t buf_phase = 0;
+        const int nblock = SWAPPED ? a0 / BK : b0 / BK;                  // tiles of at most 128 features lie in one block of the weight
+        const float* ws = p.ws + (size_t)nblock * p.kblocks;
+        const float* xs = p.xs + (size_t)(a0 + row < p.M ? a0 + row : p.M - 1) * p.kblocks;       // plain
+        float factor = 0.0f;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (SWAPPED) {
+                // the factors of the next blocks of K: [block][token], each the product of both scales
+                if ((kb - kb0) % SCALE_BLOCKS == 0) {
+                    const int t = threadIdx.x - 64, some = min(SCALE_BLOCKS, kb1 - kb);
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    for (int i = t; i < some * BN; i += 128) {
+                        const int token = i / some, b = i % some;
+                        scales[b * BN + token] = b0 + token < p.M ? p.xs[(size_t)(b0 + token) * p.kblocks + kb + b] * ws[kb + b] : 0.0f;
+                    }
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                }
+            } else {
+                factor = xs[kb] * ws[kb];
+            }
+            ok = ok && wait(&acc_full[buf], buf_phase, p.error_flag, PH_ERR_FP8_EPILOGUE);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+                tc_fence_after();
+                const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN);
+                const float* f = scales + ((kb - kb0) % SCALE_BLOCKS) * BN;
+#pragma unroll
+                for (int c = 0; c < BN; c += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(taddr + c, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(r[j]), SWAPPED ? f[c + j] : factor, acc[c + j]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(&acc_empty[buf]);
+            }
+            if (++buf == BUFFERS) { buf = 0; buf_phase ^= 1; }
+        }
+    }
+    // the sums, [column][row], into the ring's memory: every copy has landed and every product has read it
+    __syncthreads();
+    if (warp >= 2) {
+        const int row = (warp & 3) * 32 + lane;
+#pragma unroll
+        for (int j = 0; j < BN; ++j) sums[j * (BM + 1) + row] = acc[j];
+    }
+    if (splits > 1) cluster_sync_all();
+    else __syncthreads();
+    // this CTA's share of the tile: columns of the narrow side, a range for each rank
+    if (warp == 0) pdl_wait();                                           // (the other lanes of the copying warp have not waited yet)
+    if (warp == 1) pdl_wait();
+    if (SWAPPED) {
+        const int c0 = BN * rank / splits, c1 = BN * (rank + 1) / splits;
+        for (int i = threadIdx.x; i < (c1 - c0) * BM; i += THREADS) {
+            const int c = c0 + i / BM, row = i % BM, token = b0 + c, n = a0 + row;
+            if (token >= p.M || n >= p.N) continue;
+            float v = sums[c * (BM + 1) + row];
+            if (splits > 1) {
+                v = 0.0f;
+                for (int s = 0; s < splits; ++s) v += cluster_load(&sums[c * (BM + 1) + row], (uint32_t)s);
+            }
+            if (p.out_bf16) ((__nv_bfloat16*)p.out)[(size_t)token * p.N + n] = __float2bfloat16_rn(v);
+            else ((float*)p.out)[(size_t)token * p.N + n] = v;
+        }
+    } else {
+        const int r0 = BM * rank / splits, r1 = BM * (rank + 1) / splits;
+        for (int i = threadIdx.x; i < (r1 - r0) * BN; i += THREADS) {
+            const int row = r0 + i / BN, c = i % BN, token = a0 + row, n = b0 + c;
+            if (token >= p.M || n >= p.N) continue;
+            float v = sums[c * (BM + 1) + row];
+            if (splits > 1) {
+                v = 0.0f;
+                for (int s = 0; s < splits; ++s) v += cluster_load(&sums[c * (BM + 1) + row], (uint32_t)s);
+            }
+            if (p.out_bf16) ((__nv_bfloat16*)p.out)[(size_t)token * p.N + n] = __float2bfloat16_rn(v);
+            else ((float*)p.out)[(size_t)token * p.N + n] = v;
+        }
+    }
+    tc_fence_before();
+    if (splits > 1) cluster_sync_all();                                  // nobody leaves while others read its sums
+    else __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+}
+
+// ---- host side ---------------------------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiledFn)f;
+    });
+    return fn;
+}
+
+// A [rows, K] matrix of bytes seen as boxes of box_rows x 128, 128-byte swizzle, zeros outside.
+bool make_map(CUtensorMap* out, const void* ptr, int rows, int K, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)K};
+    const cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+    const cuuint32_t elem[2] = {1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, bool SWAPPED>
+int launch(const void* x, const void* w, Params p, int K, cudaStream_t stream) {
+    using Cfg = Tile<BN>;
+    constexpr auto kernel = gemm_fp8_kernel<BN, SWAPPED>;
+    if (const int rc = allow_shared<kernel>(Cfg::SMEM_BYTES, "gemm_fp8")) return rc;
+    const int rows_a = SWAPPED ? p.N : p.M, rows_b = SWAPPED ? p.M : p.N;
+    CUtensorMap ma, mb;
+    if (!make_map(&ma, SWAPPED ? w : x, rows_a, K, BM) || !make_map(&mb, SWAPPED ? x : w, rows_b, K, BN))
+        return fail(PH_ERR_LAUNCH, "gemm_fp8: cuTensorMapEncodeTiled failed (M %d, N %d, K %d)", p.M, p.N, K);
+    p.a_tiles = (rows_a + BM - 1) / BM;
+    const long long ctas = (long long)p.a_tiles * ((rows_b + BN - 1) / BN) * p.splits;
+    if (ctas > 0x7fffffffLL) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: %d x %d has too many tiles", p.M, p.N);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    // A cluster is launched in plain stream order; a CTA alone may start under the kernel in front.
+    if (p.splits > 1) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = p.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+    } else {
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    }
+    cfg.attrs = attr;
+    cudaLaunchKernelEx(&cfg, kernel, ma, mb, p);
+    return check_launch("gemm_fp8");
+}
+
+// How many CTAs share a tile's K: rounds of the CTAs over the device's places times (blocks of K of each + what a CTA costs
+// beside them), the fewest among equals.
+int choose_splits(int tiles, int kblocks, int slots) {
+    int best = 1;
+    double best_cost = -1.0;
+    for (int s = 1; s <= MAX_CLUSTER && s <= kblocks; ++s) {
+        const double cost = ((long long)tiles * s + slots - 1) / slots * ((kblocks + s - 1) / s + 4.0 + (s > 1 ? 2.0 : 0.0));
+        if (best_cost < 0 || cost < best_cost - 1e-9) { best = s; best_cost = cost; }
+    }
+    return best;
+}
+
+}  // namespace
+
+// out [M, N] (float32 or bfloat16) = x times w transposed, with scales (above); xs [M, ceil(K / 128)], ws [ceil(N / 128), ceil(K / 128)].
+// kind: 0 chooses the tile; 16, 32, 64: swapped, that many tokens on the narrow side; 128: plain, 128 x 128.  splits: 0 chooses, or the CTAs
+// (1 to 8) that share a tile's K.  early_w: w and ws are not results of a kernel that may still run when this one starts, and the first tiles of w may
+// be read before the kernel in front has ended.
+PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int M, int N, int K, int kind,
+                          int splits, int early_w, int* error_flag, cudaStream_t stream) {
+    if (M == 0) return PH_OK;
+    if (!x || !xs || !w || !ws || !out || !error_flag || M < 1 || N < 1 || K < 1 || !valid_dtype(out_dtype) || splits < 0 || splits > MAX_CLUSTER)
+        return fail(PH_ERR_ARG, "gemm_fp8: bad arguments (M %d, N %d, K %d, splits %d)", M, N, K, splits);
+    if (K % 16) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: K = %d must be a multiple of 16 (16-byte rows for TMA)", K);
+    if (((uintptr_t)x | (uintptr_t)w) & 15) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: operands must be 16-byte aligned");
+    Params p = {};
+    p.xs = xs; p.ws = ws; p.out = out; p.out_bf16 = out_dtype == PH_BF16; p.M = M; p.N = N; p.kblocks = (K + BK - 1) / BK;
+    p.early_w = early_w; p.error_flag = error_flag;
+    if (splits > p.kblocks) return fail(PH_ERR_ARG, "gemm_fp8: %d splits for %d blocks of K", splits, p.kblocks);
+    if (kind == 0) kind = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    const int narrow = kind == 128 ? N : M;
+    const int tiles = (int)std::min<long long>((long long)(((kind == 128 ? M : N) + BM - 1) / BM) * ((narrow + kind - 1) / kind), 1 << 24);
+    p.splits = splits ? splits : choose_splits(tiles, p.kblocks, multiprocessors() * (kind <= 64 ? 2 : 1));
+    switch (kind) {
+        case 16: return launch<16, true>(x, w, p, K, stream);
+        case 32: return launch<32, true>(x, w, p, K, stream);
+        case 64: return launch<64, true>(x, w, p, K, stream);
+        case 128: return launch<128, false>(x, w, p, K, stream);
+        default: return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 128", kind);
+    }
+}

@@ -1,0 +1,373 @@
+// Rows and weights in 8 bits (e4m3) with a float32 scale for each block, and the two passes that give such rows: the
+// norm behind the residual's addition, and the gated activation.
+//
+// A block is 128 values of a row (the last one of a row may be shorter), or 128 x 128 values of a weight.  With amax the
+// block's largest magnitude and a = max(amax, 448 * 2^-126): scale = a / 448, q = e4m3(x * (448 / a)), rounded to nearest,
+// ties to even.  The lower bound keeps both quotients finite for blocks of zeros and of the smallest numbers; a value that is
+// no number makes its block's scale and values none, an infinite one makes the scale infinite, so that neither is lost.
+// Everything in front of the rounding to 8 bits is float32.
+//
+// Half a warp owns a block of a row: 16 lanes of 8 values, read as 16-byte vectors (two for float32) and written as 8 bytes
+// a lane, the largest magnitude found by four exchanges.  Where rows do not lie on such boundaries (an odd width, a stride or
+// a base that is no multiple of 16 bytes) the lanes take every 16th value instead, one by one.  All three passes are bound by
+// memory: each input is read once and held in registers until its block's scale is known.
+// The reference's counterpart is its 8-bit activation blocks (src/matvec_q.hip), whose scales are per 32 values.
+#include "common.cuh"
+
+#include <cuda_fp8.h>
+
+namespace {
+
+using namespace ph;
+
+constexpr int BLOCK = 128;
+constexpr float TOP = 448.0f;                                  // the largest e4m3 value
+constexpr float LEAST = 448.0f * 1.17549435e-38f;              // 448 * 2^-126
+
+// max and min that keep what is no number
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The largest magnitude over the 16 lanes that share a block.
+__device__ __forceinline__ float half_warp_max(float v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// Two values to e4m3, the first in the low byte.
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+// The place of a lane's value i inside its block.
+template <bool VEC> __device__ __forceinline__ int place(int lane16, int i) { return VEC ? lane16 * 8 + i : lane16 + 16 * i; }
+
+// A lane's eight values of the block that starts at column k0 of a row of K (zeros behind the row's end).
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_block(const T* row, int k0, int lane16, int K, float* v) {
+    if (VEC) {
+        if (k0 + lane16 * 8 < K) load8(row + k0 + lane16 * 8, v);
+        else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int k = k0 + place<false>(lane16, i);
+            v[i] = k < K ? to_float<T>(row[k]) : 0.0f;
+        }
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_block(uint8_t* row, int k0, int lane16, int K, const float* v, float inverse) {
+    uint32_t p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = pack2(v[2 * i] * inverse, v[2 * i + 1] * inverse);
+    if (VEC) {
+        if (k0 + lane16 * 8 < K) *(uint2*)(row + k0 + lane16 * 8) = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int k = k0 + place<false>(lane16, i);
+            if (k < K) row[k] = (uint8_t)(p[i >> 1] >> (8 * (i & 1)));
+        }
+    }
+}
+
+// A lane's share of a block is in v: the block's scale to *scale, its values to q.  Every lane of the warp calls this.
+template <bool VEC>
+__device__ __forceinline__ void finish_block(uint8_t* row, float* scale, bool live, int k0, int lane16, int K, const float* v) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
+    const float a = max_nan(half_warp_max(m), LEAST);
+    if (!live) return;
+    if (lane16 == 0) *scale = a / TOP;
+    store_block<VEC>(row, k0, lane16, K, v, TOP / a);
+}
+
+constexpr int ROW_THREADS = 256;
+
+// U blocks of a row (or of several rows) for each half warp, all of them asked for before the first is worked on.
+template <typename T, bool VEC, int U>
+__global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __restrict__ x, long long stride, uint8_t* __restrict__ q, float* __restrict__ scales, long long blocks,
+                                     int kblocks, int K) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane16 = threadIdx.x & 15;
+    const long long first = ((long long)blockIdx.x * (ROW_THREADS / 16) + (threadIdx.x >> 4)) * U;
+    float v[U][8];
+    long long row[U];
+    int k0[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long b = first + u < blocks ? first + u : blocks - 1;
+        row[u] = b / kblocks;
+        k0[u] = (int)(b - row[u] * kblocks) * BLOCK;
+        load_block<VEC>(x + row[u] * stride, k0[u], lane16, K, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        finish_block<VEC>(q + row[u] * K, scales + first + u, first + u < blocks, k0[u], lane16, K, v[u]);
+}
+
+// One CTA for each 128 x 128 block of a weight: 16 half warps, eight rows each.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, long long stride, uint8_t* __restrict__ q, float* __restrict__ scales, int T_rows, int K) {
+    __shared__ float part[8];
+    pdl_wait();
+    const int lane16 = threadIdx.x & 15, half = threadIdx.x >> 4;
+    const int k0 = blockIdx.x * BLOCK;
+    const long long t0 = (long long)blockIdx.y * BLOCK;
+    float v[8][8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const long long t = t0 + r * 16 + half;
+        load_block<VEC>(x + (t < T_rows ? t : 0) * stride, k0, lane16, t < T_rows ? K : 0, v[r]);
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[r][i]));
+    m = half_warp_max(m);
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max_nan(m, part[w]);
+    const float a = max_nan(m, LEAST);
+    if (threadIdx.x == 0) scales[(long long)blockIdx.y * gridDim.x + blockIdx.x] = a / TOP;
+    const float inverse = TOP / a;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const long long t = t0 + r * 16 + half;
+        if (t < T_rows) store_block<VEC>(q + t * K, k0, lane16, K, v[r], inverse);
+    }
+}
+
+// v = x[t] + sum over the parts of add[s][t]; v to x_out[t] (or nowhere); y = v * rsqrt(mean(v^2) + eps) * weight to 8 bits.
+// One CTA a row, U blocks for each half warp.
+struct NormParams {
+    const float* x;
+    const void* add;
+    int parts;
+    long long part_stride;
+    const float* weight;
+    float eps;
+    const int32_t* rows;         // row r of the output is row rows[r] of the input (null: r); a row outside 0 .. T - 1 is left out
+    int T, E, kblocks;
+    float* x_out;
+    uint8_t* q;
+    float* scales;
+};
+
+template <typename A, bool VEC, int U, int THREADS>
+__global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(NormParams p) {
+    __shared__ float scratch[32];
+    const int lane16 = threadIdx.x & 15, half = threadIdx.x >> 4, halves = blockDim.x >> 4;
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long r = blockIdx.x;
+    const long long t = p.rows ? p.rows[r] : r;
+    if (t < 0 || t >= p.T) return;                     // the whole CTA
+    const float* x = p.x + t * p.E;
+    const A* add = (const A*)p.add + t * p.E;
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_block<VEC>(x, (half + u * halves) * BLOCK, lane16, p.E, v[u]);
+    if (p.add) {
+        for (int s = 0; s < p.parts; ++s) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float a[8];
+                load_block<VEC>(add + s * p.part_stride, (half + u * halves) * BLOCK, lane16, p.E, a);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[u][i] += a[i];
+            }
+        }
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += v[u][i] * v[u][i];
+    if (p.x_out) {
+        float* o = p.x_out + t * p.E;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k0 = (half + u * halves) * BLOCK;
+            if (VEC) {
+                if (k0 + lane16 * 8 < p.E) store8(o + k0 + lane16 * 8, v[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (k0 + place<false>(lane16, i) < p.E) o[k0 + place<false>(lane16, i)] = v[u][i];
+            }
+        }
+    }
+    const float f = rsqrtf(block_sum_any(ss, scratch) / (float)p.E + p.eps);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int b = half + u * halves;
+        float w[8];
+        load_block<VEC>(p.weight, b * BLOCK, lane16, p.E, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[u][i] = v[u][i] * f * w[i];
+        finish_block<VEC>(p.q + r * p.E, p.scales + r * p.kblocks + b, b < p.kblocks, b * BLOCK, lane16, p.E, v[u]);
+    }
+}
+
+// The gated activation of a (gate, up) pair.  kind 0: silu(g) * u; 1 clamped swish: g' = min(g, limit), u' = clamp(u, -limit,
+// limit), g' * sigmoid(alpha g') * (u' + shift); 2: gelu(g) * u in the tanh form, 0.5 g (1 + tanh(y)) = g sigmoid(2 y),
+// y = sqrt(2/pi) (g + 0.044715 g^3).
+struct Gate {
+    int kind;
+    float alpha, limit, shift;
+};
+__device__ __forceinline__ float gated_value(const Gate& gate, float g, float u) {
+    if (gate.kind == 0) return __fdividef(g, 1.0f + __expf(-g)) * u;
+    if (gate.kind == 2) return __fdividef(g, 1.0f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g))) * u;
+    g = min_nan(g, gate.limit);
+    u = min_nan(max_nan(u, -gate.limit), gate.limit);
+    return __fdividef(g, 1.0f + __expf(-gate.alpha * g)) * (u + gate.shift);
+}
+
+// Rows of (g0, u0, g1, u1, ...), in `parts` parts that are summed first, to gated rows of F in 8 bits.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restrict__ gate_up, int parts, long long part_stride, uint8_t* __restrict__ q, float* __restrict__ scales,
+                                 long long blocks, int kblocks, int F, Gate gate) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane16 = threadIdx.x & 15;
+    const long long b = (long long)blockIdx.x * (ROW_THREADS / 16) + (threadIdx.x >> 4);
+    const long long at = b < blocks ? b : blocks - 1;
+    const long long row = at / kblocks;
+    const int k0 = (int)(at - row * kblocks) * BLOCK;
+    const T* src = gate_up + row * 2 * F;
+    float h[8];
+    if (VEC) {
+        float g[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) g[i] = 0.0f;
+        if (k0 + lane16 * 8 < F) {
+            for (int s = 0; s < parts; ++s) {
+                float a[16];
+                load8(src + s * part_stride + 2 * (k0 + lane16 * 8), a);
+                load8(src + s * part_stride + 2 * (k0 + lane16 * 8) + 8, a + 8);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) g[i] = s == 0 ? a[i] : g[i] + a[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = gated_value(gate, g[2 * i], g[2 * i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int k = k0 + place<false>(lane16, i);
+            float g = 0.0f, u = 0.0f;
+            if (k < F) {
+                g = to_float<T>(src[2 * k]); u = to_float<T>(src[2 * k + 1]);
+                for (int s = 1; s < parts; ++s) { g += to_float<T>(src[s * part_stride + 2 * k]); u += to_float<T>(src[s * part_stride + 2 * k + 1]); }
+            }
+            h[i] = gated_value(gate, g, u);
+        }
+    }
+    finish_block<VEC>(q + row * F, scales + b, b < blocks, k0, lane16, F, h);
+}
+
+inline bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+template <typename A, bool VEC>
+int launch_norm(const NormParams& p, int n, cudaStream_t stream) {
+    // blocks per half warp: as few as a CTA of 512 threads allows where rows are few, so that a row is spread wide
+    const int u = p.kblocks <= 32 ? 1 : p.kblocks <= 64 ? 2 : p.kblocks <= 128 ? 4 : 8;
+    const int halves = (p.kblocks + u - 1) / u;
+    const int threads = (halves * 16 + 31) / 32 * 32;
+    switch (u) {
+        case 1: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 1, 512>, dim3(n), dim3(threads), 0, stream, p); break;
+        case 2: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 2, 512>, dim3(n), dim3(threads), 0, stream, p); break;
+        case 4: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 4, 512>, dim3(n), dim3(threads), 0, stream, p); break;
+        default: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 8, 512>, dim3(n), dim3(threads), 0, stream, p); break;
+    }
+    return check_launch("add_rmsnorm_fp8");
+}
+
+}  // namespace
+
+// x [T, K] in rows of `stride` elements to q [T, K] and scales [ceil(T / block_rows), ceil(K / 128)]; block_rows 1 or 128.
+PH_EXPORT int ph_quantize_fp8(const void* x, int dtype, long long stride, void* q, float* scales, int T, int K, int block_rows, cudaStream_t stream) {
+    if (T == 0) return PH_OK;
+    if (!x || !q || !scales || T < 0 || K < 1 || stride < K || !valid_dtype(dtype)) return fail(PH_ERR_ARG, "quantize_fp8: bad arguments (T %d, K %d, row stride %lld)", T, K, stride);
+    if (block_rows != 1 && block_rows != BLOCK) return fail(PH_ERR_ARG, "quantize_fp8: blocks are of 1 or 128 rows, not %d", block_rows);
+    const int kblocks = (K + BLOCK - 1) / BLOCK;
+    const int size = dtype == PH_F32 ? 4 : 2;
+    const bool vec = K % 8 == 0 && (stride * size) % 16 == 0 && aligned(x, 16) && aligned(q, 8);
+    if (block_rows == BLOCK) {
+        if ((T + BLOCK - 1) / BLOCK > 65535) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: a weight of at most 65535 * 128 rows, not %d", T);
+        const dim3 grid(kblocks, (T + BLOCK - 1) / BLOCK);
+        PH_DISPATCH(dtype, X, {
+            if (vec) launch_overlapped(quantize_blocks_kernel<X, true>, grid, dim3(256), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, T, K);
+            else launch_overlapped(quantize_blocks_kernel<X, false>, grid, dim3(256), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, T, K);
+        });
+        return check_launch("quantize_fp8");
+    }
+    const long long blocks = (long long)T * kblocks;
+    const long long grid = (blocks + ROW_THREADS / 16 - 1) / (ROW_THREADS / 16);
+    if (grid > 0x7fffffffLL) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: %lld blocks are too many", blocks);
+    PH_DISPATCH(dtype, X, {
+        if (vec) launch_overlapped(quantize_rows_kernel<X, true, 1>, dim3((unsigned)grid), dim3(ROW_THREADS), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, blocks, kblocks, K);
+        else launch_overlapped(quantize_rows_kernel<X, false, 1>, dim3((unsigned)grid), dim3(ROW_THREADS), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, blocks, kblocks, K);
+    });
+    return check_launch("quantize_fp8");
+}
+
+// x [T, E] float32 += the parts of add ([parts][T, E], part_stride elements apart; null: nothing), kept in x_out [T, E] (x itself, another
+// array or null); the normed rows to q [n, E] and scales [n, ceil(E / 128)].  rows [n] (or null): which rows, in that order.
+PH_EXPORT int ph_add_rmsnorm_fp8(const float* x, const void* add, int add_dtype, int parts, long long part_stride, const float* weight, float eps,
+                                 const int32_t* rows, int n, int T, int E, float* x_out, void* q, float* scales, cudaStream_t stream) {
+    if (n == 0) return PH_OK;
+    if (!x || !weight || !q || !scales || n < 0 || T < 1 || E < 1 || parts < 1 || !valid_dtype(add_dtype) || !(eps >= 0.0f))
+        return fail(PH_ERR_ARG, "add_rmsnorm_fp8: bad arguments (T %d, E %d, rows %d, parts %d, eps %g)", T, E, n, parts, (double)eps);
+    if (rows && x_out) return fail(PH_ERR_ARG, "add_rmsnorm_fp8: the sums of picked rows are not kept");
+    const int kblocks = (E + BLOCK - 1) / BLOCK;
+    if (kblocks > 256) return fail(PH_ERR_UNSUPPORTED, "add_rmsnorm_fp8: rows of at most 32768 values, not %d", E);
+    NormParams p = {x, add, parts, part_stride, weight, eps, rows, T, E, kblocks, x_out, (uint8_t*)q, scales};
+    const int size = add_dtype == PH_F32 ? 4 : 2;
+    const bool vec = E % 8 == 0 && aligned(x, 16) && aligned(weight, 16) && aligned(x_out, 16) && aligned(q, 8) && aligned(add, 16) && (part_stride * size) % 16 == 0;
+    PH_DISPATCH(add_dtype, A, { return vec ? launch_norm<A, true>(p, n, stream) : launch_norm<A, false>(p, n, stream); });
+}
+
+// gate_up [parts][T, 2 F] (part_stride elements apart) of (gate, up) pairs to q [T, F] and scales [T, ceil(F / 128)].  gate: null
+// (silu), or four floats on the host: alpha, limit, shift and the kind (1 clamped swish, 2 the tanh form of gelu).
+PH_EXPORT int ph_gated_fp8(const void* gate_up, int dtype, int parts, long long part_stride, void* q, float* scales, int T, int F, const float* gate,
+                           cudaStream_t stream) {
+    if (T == 0) return PH_OK;
+    if (!gate_up || !q || !scales || T < 0 || F < 1 || F > 0x3fffffff || parts < 1 || !valid_dtype(dtype)) return fail(PH_ERR_ARG, "gated_fp8: bad arguments (T %d, F %d, parts %d)", T, F, parts);
+    Gate g = {0, 1.0f, 0.0f, 0.0f};
+    if (gate) g = Gate{(int)gate[3], gate[0], gate[1], gate[2]};
+    if (g.kind < 0 || g.kind > 2) return fail(PH_ERR_ARG, "gated_fp8: gate %d is not known", g.kind);
+    const int kblocks = (F + BLOCK - 1) / BLOCK, size = dtype == PH_F32 ? 4 : 2;
+    const long long blocks = (long long)T * kblocks, grid = (blocks + ROW_THREADS / 16 - 1) / (ROW_THREADS / 16);
+    if (grid > 0x7fffffffLL) return fail(PH_ERR_UNSUPPORTED, "gated_fp8: %lld blocks are too many", blocks);
+    const bool vec = F % 8 == 0 && aligned(gate_up, 16) && aligned(q, 8) && (part_stride * size) % 16 == 0;
+    PH_DISPATCH(dtype, X, {
+        if (vec) launch_overlapped(gated_fp8_kernel<X, true>, dim3((unsigned)grid), dim3(ROW_THREADS), 0, stream, (const X*)gate_up, parts, part_stride, (uint8_t*)q, scales, blocks, kblocks, F, g);
+        else launch_overlapped(gated_fp8_kernel<X, false>, dim3((unsigned)grid), dim3(ROW_THREADS), 0, stream, (const X*)gate_up, parts, part_stride, (uint8_t*)q, scales, blocks, kblocks, F, g);
+    });
+    return check_launch("gated_fp8");
+}
+
+PH_DEFINE_LAST_ERROR(ph_fp8)
