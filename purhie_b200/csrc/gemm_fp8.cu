@@ -52,8 +52,13 @@ struct Params {
     int kblocks;
     int a_tiles, splits;
     int early_w;
+    int tma_store;               // pairs: 1 the copy engine stores bfloat16 boxes of 64 columns, 2 float32 boxes of 32; 0 the threads store
     int* error_flag;
 };
+
+// Where a wait that ran out is noted when the caller has no place of its own for it (one for each device).
+__device__ int g_error;
+__device__ __forceinline__ int* error_word(const Params& p) { return p.error_flag ? p.error_flag : &g_error; }
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c_inner, int c_row) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -150,6 +155,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
+    int* flag = error_word(p);
     const int splits = p.splits, rank = blockIdx.x % splits, tile = blockIdx.x / splits;
     const int a0 = (tile % p.a_tiles) * BM, b0 = (tile / p.a_tiles) * BN;
     const int kb0 = (int)((long long)p.kblocks * rank / splits), kb1 = (int)((long long)p.kblocks * (rank + 1) / splits);
@@ -175,7 +181,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             uint32_t phase = pre == STAGES ? 1 : 0;
             bool ok = true;
             for (int kb = kb0 + pre; kb < kb1; ++kb) {
-                if (!wait(&empty[stage], phase ^ 1, p.error_flag, PH_ERR_FP8_PRODUCER)) { ok = false; break; }
+                if (!wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) { ok = false; break; }
                 arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
                 tma_load_2d(smem_a + stage * A_BYTES, &map_a, &full[stage], kb * BK, a0);
                 tma_load_2d(smem_b + stage * BN * BK, &map_b, &full[stage], kb * BK, b0);
@@ -183,7 +189,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             }
             // not past this point while copies may be in flight: the products have released every stage
             for (int s = 0; s < STAGES && ok; ++s) {
-                if (!wait(&empty[stage], phase ^ 1, p.error_flag, PH_ERR_FP8_PRODUCER)) break;
+                if (!wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) break;
                 if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
         }
@@ -194,8 +200,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             int stage = 0, buf = 0;
             uint32_t phase = 0, buf_phase = 0;
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!wait(&acc_empty[buf], buf_phase ^ 1, p.error_flag, PH_ERR_FP8_MMA)) break;
-                if (!wait(&full[stage], phase, p.error_flag, PH_ERR_FP8_MMA)) break;
+                if (!wait(&acc_empty[buf], buf_phase ^ 1, flag, PH_ERR_FP8_MMA)) break;
+                if (!wait(&full[stage], phase, flag, PH_ERR_FP8_MMA)) break;
                 tc_fence_after();
                 const uint64_t adesc = smem_desc(smem_a + stage * A_BYTES), bdesc = smem_desc(smem_b + stage * BN * BK);
 #pragma unroll
@@ -236,7 +242,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             } else {
                 factor = xs[kb] * ws[kb];
             }
-            ok = ok && wait(&acc_full[buf], buf_phase, p.error_flag, PH_ERR_FP8_EPILOGUE);
+            ok = ok && wait(&acc_full[buf], buf_phase, flag, PH_ERR_FP8_EPILOGUE);
             ok = __all_sync(0xffffffffu, ok);
             if (ok) {
                 tc_fence_after();
@@ -302,6 +308,253 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     if (warp == 1) tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
 }
 
+// ---- two CTAs on one tile (cta_group::2) ---------------------------------------------------------------
+//
+// Many tokens: a cluster of two CTAs, on the two SMs of a pair, works on tiles of 256 tokens x 256 features, one pair per two
+// SMs, tile after tile.  Each CTA copies its own 128 rows of x and 128 rows of w for a block of K, half of what a CTA alone
+// would read from shared memory per product; the leader (rank 0) issues the products with M = 256, N = 256, which leave each
+// CTA its own 128 tokens x 256 features in its tensor memory: two accumulators of 256 columns, all of it.  Eight epilogue warps, two for
+// each quarter of the rows, keep the float32 sums of 32 tokens x 128 features a warp in registers, 128 a thread.  A block of K
+// costs the tensor cores 512 cycles at their peak and the epilogue 256 each of tensor-memory reads and of multiply-adds
+// (half of that as pairs), so both accumulators are needed and neither side waits for long.
+//   full[s]      in the leader: the copies of both CTAs complete there, the leader's thread announces the bytes of both;
+//   empty[s]     in each CTA: the leader's tcgen05.commit reaches both (the commit's own multicast; no load is multicast);
+//   acc_full[a]  in each CTA, by the same kind of commit; acc_empty[a] in the leader, counted in by the epilogue warps of both.
+constexpr int PAIR_BN = 256;
+constexpr int PAIR_HALF = PAIR_BN / 2;
+constexpr int PAIR_STAGE_BYTES = A_BYTES + PAIR_HALF * BK;
+constexpr int PAIR_STAGES = 5;
+constexpr int PAIR_WARPS = 8;
+constexpr int PAIR_THREADS = 128 + 32 * PAIR_WARPS;
+// Registers a thread: the launch gives each of the 384 threads 168 (what 65,536 hold), the four warps of copies and products hand
+// most of theirs back and the epilogue's take them: 128 * 40 + 256 * 232 = 384 * 168.
+constexpr int PAIR_REGS = 168, PAIR_REGS_LOW = 40, PAIR_REGS_HIGH = 232;
+static_assert(128 * PAIR_REGS_LOW + 32 * PAIR_WARPS * PAIR_REGS_HIGH <= PAIR_THREADS * PAIR_REGS, "more registers than the launch has");
+constexpr int PAIR_BOX_BYTES = 32 * 128;                          // 32 rows of 128 bytes on their way out
+constexpr int PAIR_STAGING_BYTES = PAIR_WARPS * 2 * PAIR_BOX_BYTES;
+constexpr int PAIR_SMEM_BYTES = 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + PAIR_STAGING_BYTES + 256;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+    uint32_t out;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(smem_addr(p)), "r"(rank));
+    return out;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c_inner, int c_row) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(c_inner), "r"(c_row) : "memory");
+}
+__device__ __forceinline__ void umma_pair(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Arrives on the barrier at this place in both CTAs when the products issued so far are complete.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c_inner, int c_row) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(c_inner), "r"(c_row) : "memory");
+}
+// a += v * f on two values at once.
+__device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t v0, uint32_t v1, float f) {
+    asm("{\n.reg .b64 a, v, f;\nmov.b64 a, {%0, %1};\nmov.b64 v, {%2, %3};\nmov.b64 f, {%4, %4};\nfma.rn.f32x2 a, v, f, a;\nmov.b64 {%0, %1}, a;\n}"
+        : "+f"(a0), "+f"(a1) : "r"(v0), "r"(v1), "f"(f));
+}
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&h;
+}
+
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out, Params p) {
+    constexpr int STAGES = PAIR_STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* smem_a = smem;
+    uint8_t* smem_b = smem + STAGES * A_BYTES;
+    uint8_t* staging = smem + STAGES * PAIR_STAGE_BYTES;
+    uint64_t* full = (uint64_t*)(staging + PAIR_STAGING_BYTES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* acc_full = empty + STAGES;
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const bool leader = rank == 0;
+    int* flag = error_word(p);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) { init(&full[s], 1); init(&empty[s], 1); }
+        for (int a = 0; a < 2; ++a) { init(&acc_full[a], 1); init(&acc_empty[a], 2 * PAIR_WARPS); }
+        fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(2 * PAIR_BN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                                  // the peer's barriers exist before anything signals them
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int a_tiles = p.a_tiles, b_tiles = (p.N + PAIR_BN - 1) / PAIR_BN;
+    const int tiles = a_tiles * b_tiles, first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+
+    pdl_launch_dependents();
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PAIR_REGS_LOW));
+        if (threadIdx.x == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += stride) {
+                const int a0 = (t % a_tiles) * 2 * BM + (int)rank * BM, b0 = (t / a_tiles) * PAIR_BN + (int)rank * PAIR_HALF;
+                for (int kb = 0; kb < p.kblocks; ++kb) {
+                    if (!wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) { ok = false; break; }
+                    const uint32_t bar = cluster_addr(&full[stage], 0);
+                    // The leader alone announces the bytes of both; the peer's may land first (the count of bytes owed may run
+                    // negative inside a phase, which still needs the leader's arrival).
+                    if (leader) arrive_expect_tx(&full[stage], 2 * PAIR_STAGE_BYTES);
+                    tma_load_2d_pair(smem_a + stage * A_BYTES, &map_a, bar, kb * BK, a0);
+                    tma_load_2d_pair(smem_b + stage * PAIR_HALF * BK, &map_b, bar, kb * BK, b0);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                }
+            }
+            for (int s = 0; s < STAGES && ok; ++s) {                  // not past this point while copies may be in flight
+                if (!wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) break;
+                if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+        } else if (threadIdx.x == 32 && leader) {
+            constexpr uint32_t idesc = make_idesc(2 * BM, PAIR_BN);
+            int stage = 0, buf = 0;
+            uint32_t phase = 0, buf_phase = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += stride) {
+                for (int kb = 0; kb < p.kblocks; ++kb) {
+                    if (!wait(&acc_empty[buf], buf_phase ^ 1, flag, PH_ERR_FP8_MMA)) { ok = false; break; }
+                    if (!wait(&full[stage], phase, flag, PH_ERR_FP8_MMA)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t adesc = smem_desc(smem_a + stage * A_BYTES), bdesc = smem_desc(smem_b + stage * PAIR_HALF * BK);
+#pragma unroll
+                    for (int k = 0; k < BK / UMMA_K; ++k)
+                        umma_pair(tmem_base + (uint32_t)(buf * PAIR_BN), adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k > 0 ? 1u : 0u);
+                    umma_commit_pair(&empty[stage]);
+                    umma_commit_pair(&acc_full[buf]);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                    if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PAIR_REGS_HIGH));
+        const int q = warp & 3, half = (warp - 4) >> 2;               // rows 32 q .. 32 q + 31, columns 128 half .. 128 half + 127
+        uint8_t* boxes = staging + (warp - 4) * 2 * PAIR_BOX_BYTES;
+        int buf = 0;
+        uint32_t buf_phase = 0;
+        bool ok = true;
+        for (int t = first; t < tiles; t += stride) {
+            const int row0 = (t % a_tiles) * 2 * BM + (int)rank * BM + q * 32, n0 = (t / a_tiles) * PAIR_BN + half * PAIR_HALF;
+            const int row = row0 + lane;
+            const float* xs = p.xs + (size_t)min(row, p.M - 1) * p.kblocks;
+            const float* ws = p.ws + (size_t)min(n0 / BK, (p.N - 1) / BK) * p.kblocks;
+            float acc[PAIR_HALF];
+#pragma unroll
+            for (int j = 0; j < PAIR_HALF; ++j) acc[j] = 0.0f;
+            // the scales of the next four blocks of K are on their way while these four are used
+            float f0 = 0.0f, f1 = 0.0f, f2 = 0.0f, f3 = 0.0f, x4[4], w4[4];
+            const int last = p.kblocks - 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x4[i] = xs[min(i, last)]; w4[i] = ws[min(i, last)]; }
+#pragma unroll 1
+            for (int kb = 0; kb < p.kblocks; ++kb) {
+                if ((kb & 3) == 0) {
+                    f0 = x4[0] * w4[0]; f1 = x4[1] * w4[1]; f2 = x4[2] * w4[2]; f3 = x4[3] * w4[3];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { x4[i] = xs[min(kb + 4 + i, last)]; w4[i] = ws[min(kb + 4 + i, last)]; }
+                }
+                const float f = f0;
+                f0 = f1; f1 = f2; f2 = f3;
+                ok = ok && wait(&acc_full[buf], buf_phase, flag, PH_ERR_FP8_EPILOGUE);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok) {
+                    tc_fence_after();
+                    const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * PAIR_BN + half * PAIR_HALF);
+                    uint32_t r[2][16];
+                    tmem_ld16(taddr, r[0]);
+#pragma unroll
+                    for (int c = 0; c < PAIR_HALF / 16; ++c) {
+                        tmem_ld_wait();
+                        if (c + 1 < PAIR_HALF / 16) tmem_ld16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
+                        else {
+                            tc_fence_before();                        // all of it is in registers: the accumulator is free
+                            __syncwarp();
+                            if (lane == 0) arrive_cluster(cluster_addr(&acc_empty[buf], 0));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) fma2(acc[c * 16 + j], acc[c * 16 + j + 1], r[c & 1][j], r[c & 1][j + 1], f);
+                    }
+                }
+                if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+            }
+            if (row0 >= p.M || n0 >= p.N) continue;                   // the whole warp
+            if (p.tma_store) {
+                // boxes of 32 rows x 128 bytes, swizzled as the copy engine wants them (16-byte chunk ^ (row & 7)); it leaves out what
+                // lies outside of out
+                const int n_boxes = p.tma_store == 1 ? 2 : 4;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    if (b >= n_boxes) break;
+                    uint8_t* box = boxes + (b & 1) * PAIR_BOX_BYTES;
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");       // this box of two has left
+                    __syncwarp();
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        uint4 v;
+                        if (p.tma_store == 1) {
+                            const float* a = acc + (b & 1) * 64 + c * 8;
+                            v = make_uint4(bf16_pair(a[0], a[1]), bf16_pair(a[2], a[3]), bf16_pair(a[4], a[5]), bf16_pair(a[6], a[7]));
+                        } else {
+                            const float* a = acc + b * 32 + c * 4;
+                            v = make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+                        }
+                        *(uint4*)(box + lane * 128 + ((c ^ (lane & 7)) << 4)) = v;
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    const int col = n0 + b * (p.tma_store == 1 ? 64 : 32);
+                    if (lane == 0) {
+                        if (col < p.N) tma_store_2d(&map_out, box, col, row0);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");       // one group a box, stored or not: the count above goes by them
+                    }
+                }
+            } else if (row < p.M) {
+                const size_t at = (size_t)row * p.N + n0;
+#pragma unroll
+                for (int j = 0; j < PAIR_HALF; ++j)
+                    if (n0 + j < p.N) {
+                        if (p.out_bf16) ((__nv_bfloat16*)p.out)[at + j] = __float2bfloat16_rn(acc[j]);
+                        else ((float*)p.out)[at + j] = acc[j];
+                    }
+            }
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                                  // nothing of the peer may still reach this CTA
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * PAIR_BN) : "memory");
+}
+
 // ---- host side ---------------------------------------------------------------------------------------
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -329,6 +582,46 @@ bool make_map(CUtensorMap* out, const void* ptr, int rows, int K, int box_rows) 
     const cuuint32_t elem[2] = {1, 1};
     return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// out [rows, cols] seen as boxes of 32 rows x 128 bytes, 128-byte swizzle.
+bool make_out_map(CUtensorMap* out, const void* ptr, bool bf16, int rows, int cols) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const int size = bf16 ? 2 : 4;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)cols * size};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), 32};
+    const cuuint32_t elem[2] = {1, 1};
+    return fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int launch_pair(const void* x, const void* w, Params p, int K, cudaStream_t stream) {
+    if (const int rc = allow_shared<gemm_fp8_pair_kernel>(PAIR_SMEM_BYTES, "gemm_fp8_pair")) return rc;
+    CUtensorMap ma, mb, mo;
+    if (!make_map(&ma, x, p.M, K, BM) || !make_map(&mb, w, p.N, K, PAIR_HALF))
+        return fail(PH_ERR_LAUNCH, "gemm_fp8_pair: cuTensorMapEncodeTiled failed (M %d, N %d, K %d)", p.M, p.N, K);
+    // the copy engine stores where its rules allow: rows of a multiple of 16 bytes on 16-byte boundaries
+    mo = ma;
+    p.tma_store = 0;
+    if ((p.N * (p.out_bf16 ? 2LL : 4LL)) % 16 == 0 && ((uintptr_t)p.out & 15) == 0 && make_out_map(&mo, p.out, p.out_bf16, p.M, p.N)) p.tma_store = p.out_bf16 ? 1 : 2;
+    p.a_tiles = (p.M + 2 * BM - 1) / (2 * BM);
+    const long long tiles = (long long)p.a_tiles * ((p.N + PAIR_BN - 1) / PAIR_BN);
+    if (tiles > 0x3fffffffLL) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8_pair: %d x %d has too many tiles", p.M, p.N);
+    const int clusters = (int)std::min<long long>(tiles, multiprocessors() / 2);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * clusters);
+    cfg.blockDim = dim3(PAIR_THREADS);
+    cfg.dynamicSmemBytes = PAIR_SMEM_BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];                         // in plain stream order, as every cluster here
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, gemm_fp8_pair_kernel, ma, mb, mo, p);
+    return check_launch("gemm_fp8_pair");
 }
 
 template <int BN, bool SWAPPED>
@@ -379,13 +672,13 @@ int choose_splits(int tiles, int kblocks, int slots) {
 }  // namespace
 
 // out [M, N] (float32 or bfloat16) = x times w transposed, with scales (above); xs [M, ceil(K / 128)], ws [ceil(N / 128), ceil(K / 128)].
-// kind: 0 chooses the tile; 16, 32, 64: swapped, that many tokens on the narrow side; 128: plain, 128 x 128.  splits: 0 chooses, or the CTAs
-// (1 to 8) that share a tile's K.  early_w: w and ws are not results of a kernel that may still run when this one starts, and the first tiles of w may
-// be read before the kernel in front has ended.
+// kind: 0 chooses the tile; 16, 32, 64: swapped, that many tokens on the narrow side; 128: plain, 128 x 128; 256: plain, 256 x 256 on
+// pairs of CTAs.  splits: 0 chooses, or the CTAs (1 to 8) that share a tile's K (1 on pairs).  early_w: w and ws are not results of a kernel that may still run when this one starts, and the first tiles of w may
+// be read before the kernel in front has ended.  error_flag: where a wait that ran out leaves its number (null: see ph_fp8_take_error).
 PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int M, int N, int K, int kind,
                           int splits, int early_w, int* error_flag, cudaStream_t stream) {
     if (M == 0) return PH_OK;
-    if (!x || !xs || !w || !ws || !out || !error_flag || M < 1 || N < 1 || K < 1 || !valid_dtype(out_dtype) || splits < 0 || splits > MAX_CLUSTER)
+    if (!x || !xs || !w || !ws || !out || M < 1 || N < 1 || K < 1 || !valid_dtype(out_dtype) || splits < 0 || splits > MAX_CLUSTER)
         return fail(PH_ERR_ARG, "gemm_fp8: bad arguments (M %d, N %d, K %d, splits %d)", M, N, K, splits);
     if (K % 16) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: K = %d must be a multiple of 16 (16-byte rows for TMA)", K);
     if (((uintptr_t)x | (uintptr_t)w) & 15) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: operands must be 16-byte aligned");
@@ -393,7 +686,15 @@ PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const f
     p.xs = xs; p.ws = ws; p.out = out; p.out_bf16 = out_dtype == PH_BF16; p.M = M; p.N = N; p.kblocks = (K + BK - 1) / BK;
     p.early_w = early_w; p.error_flag = error_flag;
     if (splits > p.kblocks) return fail(PH_ERR_ARG, "gemm_fp8: %d splits for %d blocks of K", splits, p.kblocks);
-    if (kind == 0) kind = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    if (kind == 0) {
+        kind = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+        if (M > 128 && (long long)((M + 255) / 256) * ((N + 255) / 256) >= multiprocessors() / 2 && splits == 0) kind = 256;
+    }
+    if (kind == 256) {
+        if (splits > 1) return fail(PH_ERR_ARG, "gemm_fp8: pairs of CTAs keep K whole");
+        p.splits = 1;
+        return launch_pair(x, w, p, K, stream);
+    }
     const int narrow = kind == 128 ? N : M;
     const int tiles = (int)std::min<long long>((long long)(((kind == 128 ? M : N) + BM - 1) / BM) * ((narrow + kind - 1) / kind), 1 << 24);
     p.splits = splits ? splits : choose_splits(tiles, p.kblocks, multiprocessors() * (kind <= 64 ? 2 : 1));
@@ -402,6 +703,16 @@ PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const f
         case 32: return launch<32, true>(x, w, p, K, stream);
         case 64: return launch<64, true>(x, w, p, K, stream);
         case 128: return launch<128, false>(x, w, p, K, stream);
-        default: return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 128", kind);
+        default: return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 128, 256", kind);
     }
+}
+
+// The number that a wait which ran out has left on the current device since the last call (0: none); waits for the device.
+PH_EXPORT int ph_fp8_take_error(int* code) {
+    if (!code) return fail(PH_ERR_ARG, "fp8_take_error: no place for the number");
+    const int zero = 0;
+    if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(code, g_error, sizeof(int)) != cudaSuccess ||
+        (*code != 0 && cudaMemcpyToSymbol(g_error, &zero, sizeof(int)) != cudaSuccess))
+        return fail(PH_ERR_LAUNCH, "fp8_take_error: %s", cudaGetErrorString(cudaGetLastError()));
+    return PH_OK;
 }

@@ -46,6 +46,7 @@ REFUSED = [
     ("gate_up", lambda: fp8.gated(f32(3, 2, 64), splits=2)),
     ("gate_up", lambda: fp8.gated(f32(2, 128)[:, :64])),
     ("CUDA", lambda: fp8.gated(f32(2, 64))),
+    ("gate 'relu'", lambda: fp8._gate("relu")),
     ("float8", lambda: fp8.gemm(bf16(2, 64), f32(2, 1), e4m3(8, 64), f32(1, 1))),
     ("float8", lambda: fp8.gemm(e4m3(64, 2).t(), f32(2, 1), e4m3(8, 64), f32(1, 1))),
     ("do not fit", lambda: fp8.gemm(e4m3(2, 64), f32(2, 1), e4m3(8, 32), f32(1, 1))),

@@ -239,16 +239,15 @@ def test_product(M, N, K, out):
     x, xs, w, ws = operands(M, N, K, M + N + K)
     y = fp8.gemm(x, xs, w, ws, out_dtype=DT[out])
     check_product(y, x, xs, w, ws)
-    fp8.check_errors(DEV)
+    fp8.check_errors()
 
 
-@pytest.mark.parametrize("tile", [16, 32, 64, 128])
-@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
-@pytest.mark.parametrize("M", [1, 40, 150])
-def test_product_of_every_tile_and_split(M, splits, tile):
+@pytest.mark.parametrize("tile,splits", [(t, s) for t in (16, 32, 64, 128) for s in (1, 2, 3, 5, 8)] + [(256, 1)])
+@pytest.mark.parametrize("M,N", [(1, 200), (40, 200), (150, 200), (290, 515)])
+def test_product_of_every_tile_and_split(M, N, splits, tile):
     """Small whole numbers and scales that are powers of two: every sum is exact in float32, so every variant gives the same bits."""
     from purhie_b200.csrc import fp8
-    N, K = 200, 2064
+    K = 2064
     g = torch.Generator(device=DEV).manual_seed(splits)
     x = torch.randint(-4, 5, (M, K), generator=g, device=DEV).float().to(torch.float8_e4m3fn)
     w = torch.randint(-4, 5, (N, K), generator=g, device=DEV).float().to(torch.float8_e4m3fn)
@@ -259,7 +258,17 @@ def test_product_of_every_tile_and_split(M, splits, tile):
     want = (x.double() * spread(xs.double(), 1, M, K)) @ (w.double() * spread(ws.double(), 128, N, K)).T
     assert torch.equal(held[1:M + 1].double(), want)
     assert (held[0] == -7).all() and (held[M + 1] == -7).all()
-    fp8.check_errors(DEV)
+    fp8.check_errors()
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(256, 256, 128), (257, 264, 16), (1000, 1003, 656), (2100, 2304, 1040), (2048, 4104, 512), (5000, 1024, 400)])
+def test_product_on_pairs(M, N, K, out):
+    """More tiles than pairs and fewer, outputs that the copy engine stores and such that the threads store."""
+    from purhie_b200.csrc import fp8
+    x, xs, w, ws = operands(M, N, K, M + N + K)
+    check_product(fp8.gemm(x, xs, w, ws, out_dtype=DT[out], tile=256), x, xs, w, ws)
+    fp8.check_errors()
 
 
 def test_product_refusals():
@@ -272,6 +281,8 @@ def test_product_refusals():
         fp8.gemm(x, xs, w, ws, splits=3)
     with pytest.raises(KernelError, match="splits"):
         fp8.gemm(x, xs, w, ws, splits=9)
+    with pytest.raises(KernelError, match="pairs"):
+        fp8.gemm(x, xs, w, ws, tile=256, splits=2)
     with pytest.raises(KernelError, match="tile"):
         fp8.gemm(x, xs, w, ws, tile=48)
     with pytest.raises(KernelError, match="unsupported dtype"):
@@ -360,4 +371,4 @@ def test_feed_forward_in_graphs_and_streams():
         torch.cuda.synchronize()
         for j in range(2):
             assert torch.equal(graphs[j][1], want[i + j])
-    fp8.check_errors(DEV)
+    fp8.check_errors()
