@@ -88,6 +88,16 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
           "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+        "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr));
+}
 
 // Shared-memory matrix descriptor of a K-major tile with the 128-byte swizzle: address >> 4 in bits 0-13, groups of eight rows 1024
 // bytes apart (>> 4, bits 32-45), version 1 at bit 46, swizzle mode 2 at bits 61-63.
@@ -344,8 +354,11 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(smem_addr(p)), "r"(rank));
     return out;
 }
+// Relaxed: what it tells is that tensor memory has been read, which the tcgen05 fence in front orders; nothing in other memory is
+// handed on.  With release semantics at cluster scope a warp waits for all it has in flight, most of a microsecond for each block of
+// K: 2048 x 24576 x 4096 took 408 us.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c_inner, int c_row) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -488,19 +501,19 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 if (ok) {
                     tc_fence_after();
                     const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * PAIR_BN + half * PAIR_HALF);
-                    uint32_t r[2][16];
-                    tmem_ld16(taddr, r[0]);
+                    uint32_t r[2][32];
+                    tmem_ld32(taddr, r[0]);
 #pragma unroll
-                    for (int c = 0; c < PAIR_HALF / 16; ++c) {
+                    for (int c = 0; c < PAIR_HALF / 32; ++c) {
                         tmem_ld_wait();
-                        if (c + 1 < PAIR_HALF / 16) tmem_ld16(taddr + (c + 1) * 16, r[(c + 1) & 1]);
+                        if (c + 1 < PAIR_HALF / 32) tmem_ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
                         else {
                             tc_fence_before();                        // all of it is in registers: the accumulator is free
                             __syncwarp();
                             if (lane == 0) arrive_cluster(cluster_addr(&acc_empty[buf], 0));
                         }
 #pragma unroll
-                        for (int j = 0; j < 16; j += 2) fma2(acc[c * 16 + j], acc[c * 16 + j + 1], r[c & 1][j], r[c & 1][j + 1], f);
+                        for (int j = 0; j < 32; j += 2) fma2(acc[c * 32 + j], acc[c * 32 + j + 1], r[c & 1][j], r[c & 1][j + 1], f);
                     }
                 }
                 if (++buf == 2) { buf = 0; buf_phase ^= 1; }
