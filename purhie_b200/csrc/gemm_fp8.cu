@@ -29,7 +29,11 @@
 namespace {
 
 using namespace ph;
-using namespace ph_mbar;
+using ph_mbar::arrive;
+using ph_mbar::arrive_expect_tx;
+using ph_mbar::fence_init;
+using ph_mbar::init;
+using ph_mbar::smem_addr;
 
 constexpr int BM = 128;
 constexpr int BK = 128;                     // values (bytes) of K in a stage: one block of the scales
@@ -59,6 +63,23 @@ struct Params {
 // Where a wait that ran out is noted when the caller has no place of its own for it (one for each device).
 __device__ int g_error;
 __device__ __forceinline__ int* error_word(const Params& p) { return p.error_flag ? p.error_flag : &g_error; }
+
+// A bounded wait that looks at the clock only now and then: these waits are short and follow one another, and the clock is slow to
+// read.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* flag, int code) {
+    unsigned long long t0 = 0;
+    for (uint32_t i = 1;; ++i) {
+        if (ph_mbar::try_wait(bar, parity)) return true;
+        if ((i & 255u) == 0) {
+            const unsigned long long now = ph_mbar::global_timer();
+            if (t0 == 0) t0 = now;
+            else if (now - t0 > ph_mbar::WAIT_LIMIT_NS) {
+                atomicExch(flag, code);
+                return false;
+            }
+        }
+    }
+}
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c_inner, int c_row) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -324,25 +345,28 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 // SMs, tile after tile.  Each CTA copies its own 128 rows of x and 128 rows of w for a block of K, half of what a CTA alone
 // would read from shared memory per product; the leader (rank 0) issues the products with M = 256, N = 256, which leave each
 // CTA its own 128 tokens x 256 features in its tensor memory: two accumulators of 256 columns, all of it.  Eight epilogue warps, two for
-// each quarter of the rows, keep the float32 sums of 32 tokens x 128 features a warp in registers, 128 a thread.  A block of K
-// costs the tensor cores 512 cycles at their peak and the epilogue 256 each of tensor-memory reads and of multiply-adds
-// (half of that as pairs), so both accumulators are needed and neither side waits for long.
+// each quarter of the rows, keep the float32 sums of 32 tokens x 128 features a warp in registers, 128 a thread.
+// What bounds it: the products alone, with the sums left in tensor memory, take 64 us for 2048 x 9472 x 4096 (2,470 TFLOP/s), with
+// the accumulators read for each block 73, with the multiply-adds 79 (2,010): both sides are busy, and hand two accumulators back
+// and forth.  Four accumulators of 128 columns were slower (92: a product of 128 columns reads its rows of x again).
 //   full[s]      in the leader: the copies of both CTAs complete there, the leader's thread announces the bytes of both;
 //   empty[s]     in each CTA: the leader's tcgen05.commit reaches both (the commit's own multicast; no load is multicast);
 //   acc_full[a]  in each CTA, by the same kind of commit; acc_empty[a] in the leader, counted in by the epilogue warps of both.
 constexpr int PAIR_BN = 256;
 constexpr int PAIR_HALF = PAIR_BN / 2;
 constexpr int PAIR_STAGE_BYTES = A_BYTES + PAIR_HALF * BK;
-constexpr int PAIR_STAGES = 5;
+constexpr int PAIR_STAGES = 4;
 constexpr int PAIR_WARPS = 8;
 constexpr int PAIR_THREADS = 128 + 32 * PAIR_WARPS;
 // Registers a thread: the launch gives each of the 384 threads 168 (what 65,536 hold), the four warps of copies and products hand
 // most of theirs back and the epilogue's take them: 128 * 40 + 256 * 232 = 384 * 168.
-constexpr int PAIR_REGS = 168, PAIR_REGS_LOW = 40, PAIR_REGS_HIGH = 232;
+constexpr int PAIR_REGS = 168, PAIR_REGS_LOW = 56, PAIR_REGS_HIGH = 224;
 static_assert(128 * PAIR_REGS_LOW + 32 * PAIR_WARPS * PAIR_REGS_HIGH <= PAIR_THREADS * PAIR_REGS, "more registers than the launch has");
 constexpr int PAIR_BOX_BYTES = 32 * 128;                          // 32 rows of 128 bytes on their way out
 constexpr int PAIR_STAGING_BYTES = PAIR_WARPS * 2 * PAIR_BOX_BYTES;
-constexpr int PAIR_SMEM_BYTES = 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + PAIR_STAGING_BYTES + 256;
+constexpr int PAIR_GROUPS = 3;                                    // of four blocks of K, whose factors lie in shared memory
+constexpr int PAIR_FACTORS_BYTES = PAIR_GROUPS * 2 * 4 * BM * 4;
+constexpr int PAIR_SMEM_BYTES = 1024 + PAIR_STAGES * PAIR_STAGE_BYTES + PAIR_STAGING_BYTES + PAIR_FACTORS_BYTES + 256;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -394,11 +418,14 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     uint8_t* smem_a = smem;
     uint8_t* smem_b = smem + STAGES * A_BYTES;
     uint8_t* staging = smem + STAGES * PAIR_STAGE_BYTES;
-    uint64_t* full = (uint64_t*)(staging + PAIR_STAGING_BYTES);
+    float* factors = (float*)(staging + PAIR_STAGING_BYTES);             // [group][half][block][row]
+    uint64_t* full = (uint64_t*)(staging + PAIR_STAGING_BYTES + PAIR_FACTORS_BYTES);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + 2;
-    uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+    uint64_t* fac_full = acc_empty + 2;
+    uint64_t* fac_empty = fac_full + PAIR_GROUPS;
+    uint32_t* tmem_slot = (uint32_t*)(fac_empty + PAIR_GROUPS);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -407,6 +434,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { init(&full[s], 1); init(&empty[s], 1); }
         for (int a = 0; a < 2; ++a) { init(&acc_full[a], 1); init(&acc_empty[a], 2 * PAIR_WARPS); }
+        for (int g = 0; g < PAIR_GROUPS; ++g) { init(&fac_full[g], 2); init(&fac_empty[g], PAIR_WARPS); }
         fence_init();
     }
     if (warp == 1) {
@@ -452,17 +480,49 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             bool ok = true;
             for (int t = first; t < tiles && ok; t += stride) {
                 for (int kb = 0; kb < p.kblocks; ++kb) {
-                    if (!wait(&acc_empty[buf], buf_phase ^ 1, flag, PH_ERR_FP8_MMA)) { ok = false; break; }
-                    if (!wait(&full[stage], phase, flag, PH_ERR_FP8_MMA)) { ok = false; break; }
+                    if (!wait(&full[stage], phase, flag, PH_ERR_FP8_MMA) || !wait(&acc_empty[buf], buf_phase ^ 1, flag, PH_ERR_FP8_MMA)) { ok = false; break; }
                     tc_fence_after();
                     const uint64_t adesc = smem_desc(smem_a + stage * A_BYTES), bdesc = smem_desc(smem_b + stage * PAIR_HALF * BK);
 #pragma unroll
                     for (int k = 0; k < BK / UMMA_K; ++k)
                         umma_pair(tmem_base + (uint32_t)(buf * PAIR_BN), adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k > 0 ? 1u : 0u);
-                    umma_commit_pair(&empty[stage]);
                     umma_commit_pair(&acc_full[buf]);
+                    umma_commit_pair(&empty[stage]);
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                     if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+                }
+            }
+        } else if (warp >= 2) {
+            // Two warps look the scales up, four blocks of K at a time and some groups ahead, and leave their products in shared memory:
+            // 2048 x 9472 x 4096 takes 79 us, and 87 where the epilogue's threads load them for themselves, however far ahead.
+            const int i = threadIdx.x - 64;
+            int g = 0;
+            uint32_t g_phase = 0;
+            bool ok = true;
+            for (int t = first; t < tiles && ok; t += stride) {
+                const int row = (t % a_tiles) * 2 * BM + (int)rank * BM + i, nb = (t / a_tiles) * 2;
+                const float* x0 = p.xs + (size_t)min(row, p.M - 1) * p.kblocks;
+                const float* x1 = p.xs + (size_t)min(row + 64, p.M - 1) * p.kblocks;
+                const float* w0 = p.ws + (size_t)nb * p.kblocks;
+                const float* w1 = p.ws + (size_t)min(nb + 1, (p.N - 1) / BK) * p.kblocks;
+                for (int kb = 0; kb < p.kblocks; kb += 4) {
+                    float a[4], b[4], u[4], v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int k = min(kb + j, p.kblocks - 1);
+                        a[j] = x0[k]; b[j] = x1[k]; u[j] = w0[k]; v[j] = w1[k];
+                    }
+                    ok = wait(&fac_empty[g], g_phase ^ 1, flag, PH_ERR_FP8_EPILOGUE);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    float* f = factors + g * 2 * 4 * BM + i;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        f[j * BM] = a[j] * u[j]; f[j * BM + 64] = b[j] * u[j];
+                        f[(4 + j) * BM] = a[j] * v[j]; f[(4 + j) * BM + 64] = b[j] * v[j];
+                    }
+                    __syncwarp();
+                    if (lane == 0) arrive(&fac_full[g]);
+                    if (++g == PAIR_GROUPS) { g = 0; g_phase ^= 1; }
                 }
             }
         }
@@ -474,49 +534,58 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         int buf = 0;
         uint32_t buf_phase = 0;
         bool ok = true;
+        int group = 0;
+        uint32_t g_phase = 0;
+        const uint32_t give_0 = cluster_addr(&acc_empty[0], 0), give_1 = cluster_addr(&acc_empty[1], 0);
+        uint32_t taddr = 0;
+        // this thread's factor of block kb (each block of a tile once, in order)
+        auto next_factor = [&](int kb) {
+            if ((kb & 3) == 0) ok = ok && wait(&fac_full[group], g_phase, flag, PH_ERR_FP8_EPILOGUE);
+            const float f = factors[((group * 2 + half) * 4 + (kb & 3)) * BM + q * 32 + lane];
+            if ((kb & 3) == 3 || kb + 1 == p.kblocks) {
+                __syncwarp();
+                if (lane == 0) arrive(&fac_empty[group]);
+                if (++group == PAIR_GROUPS) { group = 0; g_phase ^= 1; }
+            }
+            return f;
+        };
+        // waits for the next accumulator and asks for its first columns
+        auto next_accumulator = [&](uint32_t* r) {
+            ok = ok && wait(&acc_full[buf], buf_phase, flag, PH_ERR_FP8_EPILOGUE);
+            __syncwarp();
+            tc_fence_after();
+            taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * PAIR_BN + half * PAIR_HALF);
+            tmem_ld32(taddr, r);
+        };
         for (int t = first; t < tiles; t += stride) {
             const int row0 = (t % a_tiles) * 2 * BM + (int)rank * BM + q * 32, n0 = (t / a_tiles) * PAIR_BN + half * PAIR_HALF;
             const int row = row0 + lane;
-            const float* xs = p.xs + (size_t)min(row, p.M - 1) * p.kblocks;
-            const float* ws = p.ws + (size_t)min(n0 / BK, (p.N - 1) / BK) * p.kblocks;
             float acc[PAIR_HALF];
 #pragma unroll
             for (int j = 0; j < PAIR_HALF; ++j) acc[j] = 0.0f;
-            // the scales of the next four blocks of K are on their way while these four are used
-            float f0 = 0.0f, f1 = 0.0f, f2 = 0.0f, f3 = 0.0f, x4[4], w4[4];
-            const int last = p.kblocks - 1;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { x4[i] = xs[min(i, last)]; w4[i] = ws[min(i, last)]; }
+            // The loads run one chunk of 32 columns ahead of the multiply-adds, over the end of a block too, and so does the factor.
+            uint32_t r[2][32];
+            float f = next_factor(0), f_next = 0.0f;
+            next_accumulator(r[0]);
 #pragma unroll 1
             for (int kb = 0; kb < p.kblocks; ++kb) {
-                if ((kb & 3) == 0) {
-                    f0 = x4[0] * w4[0]; f1 = x4[1] * w4[1]; f2 = x4[2] * w4[2]; f3 = x4[3] * w4[3];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { x4[i] = xs[min(kb + 4 + i, last)]; w4[i] = ws[min(kb + 4 + i, last)]; }
-                }
-                const float f = f0;
-                f0 = f1; f1 = f2; f2 = f3;
-                ok = ok && wait(&acc_full[buf], buf_phase, flag, PH_ERR_FP8_EPILOGUE);
-                ok = __all_sync(0xffffffffu, ok);
-                if (ok) {
-                    tc_fence_after();
-                    const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * PAIR_BN + half * PAIR_HALF);
-                    uint32_t r[2][32];
-                    tmem_ld32(taddr, r[0]);
-#pragma unroll
-                    for (int c = 0; c < PAIR_HALF / 32; ++c) {
-                        tmem_ld_wait();
-                        if (c + 1 < PAIR_HALF / 32) tmem_ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
-                        else {
-                            tc_fence_before();                        // all of it is in registers: the accumulator is free
-                            __syncwarp();
-                            if (lane == 0) arrive_cluster(cluster_addr(&acc_empty[buf], 0));
-                        }
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) fma2(acc[c * 32 + j], acc[c * 32 + j + 1], r[c & 1][j], r[c & 1][j + 1], f);
+                for (int c = 0; c < PAIR_HALF / 32; ++c) {
+                    tmem_ld_wait();
+                    if (c + 1 < PAIR_HALF / 32) {
+                        tmem_ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+                        if (c == 1 && kb + 1 < p.kblocks) f_next = next_factor(kb + 1);
+                    } else {
+                        tc_fence_before();                            // all of it is in registers: the accumulator is free
+                        __syncwarp();
+                        if (lane == 0) arrive_cluster(buf ? give_1 : give_0);
+                        if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+                        if (kb + 1 < p.kblocks) next_accumulator(r[0]);
                     }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) fma2(acc[c * 32 + j], acc[c * 32 + j + 1], r[c & 1][j], r[c & 1][j + 1], f);
                 }
-                if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+                f = f_next;
             }
             if (row0 >= p.M || n0 >= p.N) continue;                   // the whole warp
             if (p.tma_store) {
