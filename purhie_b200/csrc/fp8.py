@@ -12,6 +12,7 @@ Outputs are made when they are not given, and returned.  Given ones are contiguo
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional, Tuple
 
@@ -26,7 +27,9 @@ register_signatures("fp8", {
                            c_void_p, c_void_p],
     "ph_gated_fp8": [c_void_p, c_int, c_int, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p],
     "ph_fp8_take_error": [c_void_p],
-    "ph_gemm_fp8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+    "ph_gemm_fp8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
+                    c_void_p],
+    "ph_gemm_fp8_plan": [c_int, c_int, c_int, c_void_p, c_void_p],
 })
 
 BLOCK = 128
@@ -167,13 +170,23 @@ def check_errors() -> None:
         raise KernelError(f"gemm_fp8: {ERRORS.get(code.value, 'error')} (status {code.value})")
 
 
+@functools.lru_cache(maxsize=4096)
+def plan(M: int, N: int, K: int, device: int = 0, tile: int = 0, splits: int = 0) -> Tuple[int, int]:
+    """How a product is cut on the current device (number ``device``) where ``tile`` and ``splits`` are 0: tokens of a tile, parts of K."""
+    t, s = c_int(tile), c_int(splits)
+    call("fp8", "ph_gemm_fp8_plan", M, N, K, ctypes.addressof(t), ctypes.addressof(s))
+    return t.value, s.value
+
+
 def gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Optional[torch.Tensor] = None, *,
          out_dtype: torch.dtype = torch.bfloat16, tile: int = 0, splits: int = 0, early_w: bool = False) -> torch.Tensor:
     """out [M, N] = (x * x_scales) @ (w * w_scales)^T: x [M, K] with x_scales [M, ceil(K / 128)], w [N, K] with w_scales
     [ceil(N / 128), ceil(K / 128)], K a multiple of 16, sums in float32, out float32 or bfloat16 (``out_dtype`` where out is not
-    given).  ``tile`` and ``splits`` (0: the kernel's own choice): 16, 32 or 64 tokens beside 128 features, 128 x 128, or (256)
-    256 x 256 on pairs of CTAs; the CTAs that share a tile's K.  ``early_w``: w is not the result of a kernel that may still run when the product starts (a model's weight),
-    so its first tiles may be read before the kernel in front has ended."""
+    given).  ``splits`` > 1: K is cut into that many parts and out is [splits, M, N] float32, the sums of each, for a consumer that
+    adds them up (``add_rmsnorm``, ``gated``); 0: cut as the kernel likes it, and out is the whole sum.  ``tile`` (0: the kernel's own
+    choice): 16, 32, 64 or 128 tokens beside 128 features, or 256 x 256 on pairs of CTAs.  ``early_w``: w is not the result of a
+    kernel that may still run when the product starts (a model's weight), so its first tiles may be read before the kernel in
+    front has ended."""
     M, K = _matrix("gemm_fp8", "x", x)
     N, K2 = _matrix("gemm_fp8", "w", w)
     if x.dtype != E4M3 or w.dtype != E4M3 or not x.is_contiguous() or not w.is_contiguous():
@@ -185,9 +198,17 @@ def gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: tor
         raise KernelError(f"gemm_fp8: x_scales must be contiguous float32 [{M}, {kb}]")
     if w_scales.dtype != F32 or w_scales.shape != (_blocks(N), kb) or not w_scales.is_contiguous():
         raise KernelError(f"gemm_fp8: w_scales must be contiguous float32 [{_blocks(N)}, {kb}]")
-    code = ops._code(out_dtype if out is None else out.dtype)
+    parted = splits > 1
+    dtype = F32 if parted else out_dtype if out is None else out.dtype
+    code = ops._code(dtype)
     stream = _stream("gemm_fp8", x, x_scales, w, w_scales, out)
-    out = x.new_empty((M, N), dtype=out_dtype) if out is None else _check("gemm_fp8", "out", out, (M, N), out.dtype)
-    call("fp8", "ph_gemm_fp8", x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), code, M, N, K, tile, splits,
-         early_w, None, stream)
+    shape = (splits, M, N) if parted else (M, N)
+    out = x.new_empty(shape, dtype=dtype) if out is None else _check("gemm_fp8", "out", out, shape, dtype)
+    if not M:
+        return out
+    if not tile or not splits:
+        tile, splits = plan(M, N, K, x.get_device(), tile, splits)
+    parts = out if parted else x.new_empty((splits, M, N), dtype=F32) if splits > 1 else None
+    call("fp8", "ph_gemm_fp8", x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), None if parted else out.data_ptr(), code, M, N, K,
+         tile, splits, None if parts is None else parts.data_ptr(), early_w, None, stream)
     return out

@@ -8,14 +8,17 @@
 // warps read each block's accumulator with tcgen05.ld, multiply it by the two scales and add, while the tensor cores work on
 // the next blocks in other accumulators.  A block of K is one stage of the ring: 128 bytes a row, one row of the swizzle.
 //
-// One CTA computes a tile of 128 x BN.  Plain orientation: the 128 rows are tokens, and a thread's scale is its own row's.  Swapped
-// (few tokens): they are features of the weight, which is what has to be streamed, and the tokens lie on the narrow side; the
-// scale then differs by column and comes from shared memory.  Where the tiles are fewer than the CTAs that the device holds, K
-// is cut among the CTAs of a cluster, which leave their sums in shared memory and add them up there, in the order of their
-// ranks: one launch, no workspace, and the same bits every time.
+// One CTA computes 128 features x BN tokens: the weight, which is what has to be streamed when tokens are few, fills the 128
+// rows of the instruction, a thread's scale differs by column and comes from shared memory, and the lanes of a warp hold
+// neighbouring features, so that whole lines leave straight from the registers.  Where the tiles are fewer than the CTAs that the
+// device holds, K is cut into parts: float32 sums [part][token][feature] that whoever consumes the product adds up in order
+// (the norm and the activation take them), or a short kernel behind this one; the same bits every time.  (Cut among the CTAs of
+// a cluster that add up in shared memory, 8 x 6144 x 4096 took 16 us: a cluster starts late and not under the kernel in front.
+// With mma.sync and 16 features a CTA, K whole, 8 x 24576 x 4096 took 25 us: its 8-bit products are slow here.)
+// Many tokens: pairs of CTAs, further down.
 //
-// Every wait on an mbarrier is bounded; a wait that runs out sets *error_flag, and the CTA still takes part in the cluster's
-// barriers, frees its tensor memory and returns (what it writes is then meaningless).
+// Every wait on an mbarrier is bounded; a wait that runs out sets *error_flag, and the CTA still frees its tensor memory and
+// returns (what it writes is then meaningless).
 // The reference's counterpart is its WMMA tile kernel over 8-bit blocks (src/matvec_q.hip:3437-3547).
 #include "common.cuh"
 #include "mbarrier.cuh"
@@ -40,8 +43,8 @@ constexpr int BK = 128;                     // values (bytes) of K in a stage: o
 constexpr int UMMA_K = 32;
 constexpr int THREADS = 192;                // copies, products, four epilogue warps
 constexpr int A_BYTES = BM * BK;
-constexpr int SCALE_BLOCKS = 32;            // blocks of K whose scales lie in shared memory at a time (swapped)
-constexpr int MAX_CLUSTER = 8;
+constexpr int FACTOR_BLOCKS = 32;           // blocks of K whose factors lie in shared memory at a time
+constexpr int MAX_SPLITS = 16;
 
 #define PH_ERR_FP8_PRODUCER 131
 #define PH_ERR_FP8_MMA 132
@@ -133,46 +136,35 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The float at the place of p in the shared memory of the CTA of that rank.
-__device__ __forceinline__ float cluster_load(const float* p, uint32_t rank) {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
-
-// Few tokens: two CTAs share an SM, so that one's start and end overlap the other's streaming.
+// Few tokens (tiles of up to 64): two CTAs share an SM, so that one's start and end overlap the other's streaming.
 template <int BN> struct Tile {
     static constexpr int STAGE_BYTES = A_BYTES + BN * BK;
     static constexpr int CTAS_PER_SM = BN <= 64 ? 2 : 1;
-    static constexpr int STAGES = (CTAS_PER_SM == 2 ? 96 : 196) * 1024 / STAGE_BYTES;
+    static constexpr int STAGES = (CTAS_PER_SM == 2 ? 96 : 192) * 1024 / STAGE_BYTES;
     static constexpr int BUFFERS = BN >= 64 ? 4 : 128 / BN;              // accumulators in tensor memory
     static constexpr int TMEM_COLS = BUFFERS * BN;
-    static constexpr int SUMS_BYTES = BN * (BM + 1) * 4;                 // the tile's sums, in the ring's memory once it is empty
-    static constexpr int SCALES_BYTES = SCALE_BLOCKS * BN * 4;
-    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + SCALES_BYTES + 256;
-    static_assert(SUMS_BYTES <= STAGES * STAGE_BYTES, "the sums do not fit");
+    static constexpr int FACTORS_BYTES = FACTOR_BLOCKS * BN * 4;
+    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + FACTORS_BYTES + 256;
+    static constexpr int CHUNK = BN >= 64 ? 32 : 16;                     // columns of an accumulator that are read at a time
     static_assert(TMEM_COLS * CTAS_PER_SM <= 512, "tensor memory");
+    static_assert((2 * STAGES + 2 * BUFFERS) * 8 + 4 <= 256, "barriers");
 };
 
-template <int BN, bool SWAPPED>
+template <int BN>
 __global__ void __launch_bounds__(THREADS, Tile<BN>::CTAS_PER_SM)
-gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, Params p) {
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, Params p) {
     using Cfg = Tile<BN>;
-    constexpr int STAGES = Cfg::STAGES, BUFFERS = Cfg::BUFFERS;
+    constexpr int STAGES = Cfg::STAGES, BUFFERS = Cfg::BUFFERS, CHUNK = Cfg::CHUNK;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t* smem_a = smem;
-    uint8_t* smem_b = smem + STAGES * A_BYTES;
-    float* sums = (float*)smem;                                          // [BN][BM + 1]
-    float* scales = (float*)(smem + STAGES * Cfg::STAGE_BYTES);          // [SCALE_BLOCKS][BN], swapped
-    uint64_t* full = (uint64_t*)(smem + STAGES * Cfg::STAGE_BYTES + Cfg::SCALES_BYTES);
+    uint8_t* smem_w = smem;
+    uint8_t* smem_x = smem + STAGES * A_BYTES;
+    float* factors = (float*)(smem + STAGES * Cfg::STAGE_BYTES);         // [block][token]
+    uint64_t* full = (uint64_t*)(smem + STAGES * Cfg::STAGE_BYTES + Cfg::FACTORS_BYTES);
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + BUFFERS;
     uint32_t* tmem_slot = (uint32_t*)(acc_empty + BUFFERS);
-    static_assert((2 * STAGES + 2 * BUFFERS) * 8 + 4 <= 256, "barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -187,12 +179,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t tmem_base = *tmem_slot;
 
     int* flag = error_word(p);
-    const int splits = p.splits, rank = blockIdx.x % splits, tile = blockIdx.x / splits;
-    const int a0 = (tile % p.a_tiles) * BM, b0 = (tile / p.a_tiles) * BN;
-    const int kb0 = (int)((long long)p.kblocks * rank / splits), kb1 = (int)((long long)p.kblocks * (rank + 1) / splits);
+    const int splits = p.splits, split = blockIdx.x % splits, tile = blockIdx.x / splits;
+    const int n0 = (tile % p.a_tiles) * BM, m0 = (tile / p.a_tiles) * BN;
+    const int kb0 = (int)((long long)p.kblocks * split / splits), kb1 = (int)((long long)p.kblocks * (split + 1) / splits);
 
     pdl_launch_dependents();
-    float acc[BN];
     if (warp == 0) {
         if (lane == 0) {
             // the weight's tiles of the first stages may not have to wait for the kernel in front
@@ -200,22 +191,18 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (p.early_w)
                 for (; pre < STAGES && kb0 + pre < kb1; ++pre) {
                     arrive_expect_tx(&full[pre], Cfg::STAGE_BYTES);
-                    if (SWAPPED) tma_load_2d(smem_a + pre * A_BYTES, &map_a, &full[pre], (kb0 + pre) * BK, a0);
-                    else tma_load_2d(smem_b + pre * BN * BK, &map_b, &full[pre], (kb0 + pre) * BK, b0);
+                    tma_load_2d(smem_w + pre * A_BYTES, &map_w, &full[pre], (kb0 + pre) * BK, n0);
                 }
             pdl_wait();
-            for (int s = 0; s < pre; ++s) {
-                if (SWAPPED) tma_load_2d(smem_b + s * BN * BK, &map_b, &full[s], (kb0 + s) * BK, b0);
-                else tma_load_2d(smem_a + s * A_BYTES, &map_a, &full[s], (kb0 + s) * BK, a0);
-            }
+            for (int s = 0; s < pre; ++s) tma_load_2d(smem_x + s * BN * BK, &map_x, &full[s], (kb0 + s) * BK, m0);
             int stage = pre == STAGES ? 0 : pre;
             uint32_t phase = pre == STAGES ? 1 : 0;
             bool ok = true;
             for (int kb = kb0 + pre; kb < kb1; ++kb) {
                 if (!wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) { ok = false; break; }
                 arrive_expect_tx(&full[stage], Cfg::STAGE_BYTES);
-                tma_load_2d(smem_a + stage * A_BYTES, &map_a, &full[stage], kb * BK, a0);
-                tma_load_2d(smem_b + stage * BN * BK, &map_b, &full[stage], kb * BK, b0);
+                tma_load_2d(smem_w + stage * A_BYTES, &map_w, &full[stage], kb * BK, n0);
+                tma_load_2d(smem_x + stage * BN * BK, &map_x, &full[stage], kb * BK, m0);
                 if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
             // not past this point while copies may be in flight: the products have released every stage
@@ -224,119 +211,131 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
         }
-        __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = make_idesc(BM, BN);
             int stage = 0, buf = 0;
             uint32_t phase = 0, buf_phase = 0;
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!wait(&acc_empty[buf], buf_phase ^ 1, flag, PH_ERR_FP8_MMA)) break;
-                if (!wait(&full[stage], phase, flag, PH_ERR_FP8_MMA)) break;
+                if (!wait(&acc_empty[buf], buf_phase ^ 1, flag, PH_ERR_FP8_MMA) || !wait(&full[stage], phase, flag, PH_ERR_FP8_MMA)) break;
                 tc_fence_after();
-                const uint64_t adesc = smem_desc(smem_a + stage * A_BYTES), bdesc = smem_desc(smem_b + stage * BN * BK);
+                const uint64_t adesc = smem_desc(smem_w + stage * A_BYTES), bdesc = smem_desc(smem_x + stage * BN * BK);
 #pragma unroll
                 for (int k = 0; k < BK / UMMA_K; ++k)                    // 32 values further along the swizzled row
                     umma(tmem_base + (uint32_t)(buf * BN), adesc + (uint64_t)(k * 2), bdesc + (uint64_t)(k * 2), idesc, k > 0 ? 1u : 0u);
-                umma_commit(&empty[stage]);
                 umma_commit(&acc_full[buf]);
+                umma_commit(&empty[stage]);
                 if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 if (++buf == BUFFERS) { buf = 0; buf_phase ^= 1; }
             }
         }
-        __syncwarp();
     } else {
         const int q = warp & 3;                                          // the quarter of the accumulator's rows that this warp may read
-        const int row = q * 32 + lane;
+        const int n = n0 + q * 32 + lane;
         pdl_wait();
+        float acc[BN];
 #pragma unroll
         for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
         int buf = 0;
         uint32_t buf_phase = 0;
-        const int nblock = SWAPPED ? a0 / BK : b0 / BK;                  // tiles of at most 128 features lie in one block of the weight
-        const float* ws = p.ws + (size_t)nblock * p.kblocks;
-        const float* xs = p.xs + (size_t)(a0 + row < p.M ? a0 + row : p.M - 1) * p.kblocks;       // plain
-        float factor = 0.0f;
         bool ok = true;
-        for (int kb = kb0; kb < kb1; ++kb) {
-            if (SWAPPED) {
-                // the factors of the next blocks of K: [block][token], each the product of both scales
-                if ((kb - kb0) % SCALE_BLOCKS == 0) {
-                    const int t = threadIdx.x - 64, some = min(SCALE_BLOCKS, kb1 - kb);
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                    for (int i = t; i < some * BN; i += 128) {
-                        const int token = i / some, b = i % some;
-                        scales[b * BN + token] = b0 + token < p.M ? p.xs[(size_t)(b0 + token) * p.kblocks + kb + b] * ws[kb + b] : 0.0f;
-                    }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                }
-            } else {
-                factor = xs[kb] * ws[kb];
+        const float* ws = p.ws + (size_t)(n0 / BK) * p.kblocks;
+        for (int base = kb0; base < kb1; base += FACTOR_BLOCKS) {
+            // the factors of the next blocks of K, [block][token], each the product of both scales: a lane a block, a warp a token
+            const int some = min(FACTOR_BLOCKS, kb1 - base);
+            if (base > kb0) asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (lane < some) {
+                const float s = ws[base + lane];
+#pragma unroll 8
+                for (int token = warp - 2; token < BN; token += 4)
+                    factors[lane * BN + token] = p.xs[(size_t)min(m0 + token, p.M - 1) * p.kblocks + base + lane] * s;
             }
-            ok = ok && wait(&acc_full[buf], buf_phase, flag, PH_ERR_FP8_EPILOGUE);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            for (int b = 0; b < some; ++b) {
+                const float4* f = (const float4*)(factors + b * BN);
+                ok = ok && wait(&acc_full[buf], buf_phase, flag, PH_ERR_FP8_EPILOGUE);
+                __syncwarp();
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN);
-                const float* f = scales + ((kb - kb0) % SCALE_BLOCKS) * BN;
+                uint32_t r[2][CHUNK];
+                if constexpr (CHUNK == 32) tmem_ld32(taddr, r[0]); else tmem_ld16(taddr, r[0]);
 #pragma unroll
-                for (int c = 0; c < BN; c += 16) {
-                    uint32_t r[16];
-                    tmem_ld16(taddr + c, r);
+                for (int c = 0; c < BN / CHUNK; ++c) {
                     tmem_ld_wait();
+                    if (c + 1 < BN / CHUNK) {
+                        if constexpr (CHUNK == 32) tmem_ld32(taddr + (c + 1) * CHUNK, r[(c + 1) & 1]); else tmem_ld16(taddr + (c + 1) * CHUNK, r[(c + 1) & 1]);
+                    } else {
+                        tc_fence_before();                               // all of it is in registers: the accumulator is free
+                        __syncwarp();
+                        if (lane == 0) arrive(&acc_empty[buf]);
+                    }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(r[j]), SWAPPED ? f[c + j] : factor, acc[c + j]);
+                    for (int j = 0; j < CHUNK; j += 4) {
+                        const float4 v = f[(c * CHUNK + j) / 4];
+                        float* a = acc + c * CHUNK + j;
+                        const uint32_t* d = r[c & 1] + j;
+                        a[0] = fmaf(__uint_as_float(d[0]), v.x, a[0]); a[1] = fmaf(__uint_as_float(d[1]), v.y, a[1]);
+                        a[2] = fmaf(__uint_as_float(d[2]), v.z, a[2]); a[3] = fmaf(__uint_as_float(d[3]), v.w, a[3]);
+                    }
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) arrive(&acc_empty[buf]);
+                if (++buf == BUFFERS) { buf = 0; buf_phase ^= 1; }
             }
-            if (++buf == BUFFERS) { buf = 0; buf_phase ^= 1; }
         }
-    }
-    // the sums, [column][row], into the ring's memory: every copy has landed and every product has read it
-    __syncthreads();
-    if (warp >= 2) {
-        const int row = (warp & 3) * 32 + lane;
+        // the lanes of a warp hold neighbouring features of a token: whole lines leave straight from the registers
+        if (p.out_bf16 && splits == 1) {
+            // (two tokens at a time: the even lanes store a pair of features of the one, the odd lanes of the other)
+            const int odd = lane & 1, pair = n - odd;
+            const bool wide = (p.N & 1) == 0 && ((uintptr_t)p.out & 3) == 0;
 #pragma unroll
-        for (int j = 0; j < BN; ++j) sums[j * (BM + 1) + row] = acc[j];
-    }
-    if (splits > 1) cluster_sync_all();
-    else __syncthreads();
-    // this CTA's share of the tile: columns of the narrow side, a range for each rank
-    if (warp == 0) pdl_wait();                                           // (the other lanes of the copying warp have not waited yet)
-    if (warp == 1) pdl_wait();
-    if (SWAPPED) {
-        const int c0 = BN * rank / splits, c1 = BN * (rank + 1) / splits;
-        for (int i = threadIdx.x; i < (c1 - c0) * BM; i += THREADS) {
-            const int c = c0 + i / BM, row = i % BM, token = b0 + c, n = a0 + row;
-            if (token >= p.M || n >= p.N) continue;
-            float v = sums[c * (BM + 1) + row];
-            if (splits > 1) {
-                v = 0.0f;
-                for (int s = 0; s < splits; ++s) v += cluster_load(&sums[c * (BM + 1) + row], (uint32_t)s);
+            for (int j = 0; j < BN; j += 2) {
+                const float got = __shfl_xor_sync(0xffffffffu, odd ? acc[j] : acc[j + 1], 1);
+                const __nv_bfloat162 v = odd ? __floats2bfloat162_rn(got, acc[j + 1]) : __floats2bfloat162_rn(acc[j], got);
+                const int m = m0 + j + odd;
+                if (m >= p.M || pair >= p.N) continue;
+                __nv_bfloat16* o = (__nv_bfloat16*)p.out + (size_t)m * p.N + pair;
+                if (wide) *(__nv_bfloat162*)o = v;
+                else {
+                    o[0] = __low2bfloat16(v);
+                    if (pair + 1 < p.N) o[1] = __high2bfloat16(v);
+                }
             }
-            if (p.out_bf16) ((__nv_bfloat16*)p.out)[(size_t)token * p.N + n] = __float2bfloat16_rn(v);
-            else ((float*)p.out)[(size_t)token * p.N + n] = v;
-        }
-    } else {
-        const int r0 = BM * rank / splits, r1 = BM * (rank + 1) / splits;
-        for (int i = threadIdx.x; i < (r1 - r0) * BN; i += THREADS) {
-            const int row = r0 + i / BN, c = i % BN, token = a0 + row, n = b0 + c;
-            if (token >= p.M || n >= p.N) continue;
-            float v = sums[c * (BM + 1) + row];
-            if (splits > 1) {
-                v = 0.0f;
-                for (int s = 0; s < splits; ++s) v += cluster_load(&sums[c * (BM + 1) + row], (uint32_t)s);
-            }
-            if (p.out_bf16) ((__nv_bfloat16*)p.out)[(size_t)token * p.N + n] = __float2bfloat16_rn(v);
-            else ((float*)p.out)[(size_t)token * p.N + n] = v;
+        } else if (n < p.N) {
+            float* o = (float*)p.out + (size_t)split * p.M * p.N + (size_t)m0 * p.N + n;
+#pragma unroll
+            for (int j = 0; j < BN; ++j)
+                if (m0 + j < p.M) o[(size_t)j * p.N] = acc[j];
         }
     }
     tc_fence_before();
-    if (splits > 1) cluster_sync_all();                                  // nobody leaves while others read its sums
-    else __syncthreads();
-    if (warp == 1) tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+    }
+}
+
+// out = the sum of the parts ([parts][values] float32), in their order; four values a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ parts, int n_parts, long long values, T* __restrict__ out) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= values) return;
+    if ((values & 3) == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int s = 0; s < n_parts; ++s) {
+            const float4 a = *(const float4*)(parts + s * values + i);
+            v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        }
+        store4(out + i, v);
+    } else {
+        for (long long j = i; j < i + 4 && j < values; ++j) {
+            float v = 0.0f;
+            for (int s = 0; s < n_parts; ++s) v += parts[s * values + j];
+            out[j] = from_float<T>(v);
+        }
+    }
 }
 
 // ---- two CTAs on one tile (cta_group::2) ---------------------------------------------------------------
@@ -706,87 +705,88 @@ int launch_pair(const void* x, const void* w, Params p, int K, cudaStream_t stre
     return check_launch("gemm_fp8_pair");
 }
 
-template <int BN, bool SWAPPED>
+template <int BN>
 int launch(const void* x, const void* w, Params p, int K, cudaStream_t stream) {
     using Cfg = Tile<BN>;
-    constexpr auto kernel = gemm_fp8_kernel<BN, SWAPPED>;
-    if (const int rc = allow_shared<kernel>(Cfg::SMEM_BYTES, "gemm_fp8")) return rc;
-    const int rows_a = SWAPPED ? p.N : p.M, rows_b = SWAPPED ? p.M : p.N;
-    CUtensorMap ma, mb;
-    if (!make_map(&ma, SWAPPED ? w : x, rows_a, K, BM) || !make_map(&mb, SWAPPED ? x : w, rows_b, K, BN))
+    if (const int rc = allow_shared<gemm_fp8_kernel<BN>>(Cfg::SMEM_BYTES, "gemm_fp8")) return rc;
+    CUtensorMap mw, mx;
+    if (!make_map(&mw, w, p.N, K, BM) || !make_map(&mx, x, p.M, K, BN))
         return fail(PH_ERR_LAUNCH, "gemm_fp8: cuTensorMapEncodeTiled failed (M %d, N %d, K %d)", p.M, p.N, K);
-    p.a_tiles = (rows_a + BM - 1) / BM;
-    const long long ctas = (long long)p.a_tiles * ((rows_b + BN - 1) / BN) * p.splits;
+    p.a_tiles = (p.N + BM - 1) / BM;
+    const long long ctas = (long long)p.a_tiles * ((p.M + BN - 1) / BN) * p.splits;
     if (ctas > 0x7fffffffLL) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: %d x %d has too many tiles", p.M, p.N);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    // A cluster is launched in plain stream order; a CTA alone may start under the kernel in front.
-    if (p.splits > 1) {
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = p.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-        cfg.numAttrs = 1;
-    } else {
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    }
-    cfg.attrs = attr;
-    cudaLaunchKernelEx(&cfg, kernel, ma, mb, p);
+    launch_overlapped(gemm_fp8_kernel<BN>, dim3((unsigned)ctas), dim3(THREADS), Cfg::SMEM_BYTES, stream, mw, mx, p);
     return check_launch("gemm_fp8");
 }
 
-// How many CTAs share a tile's K: rounds of the CTAs over the device's places times (blocks of K of each + what a CTA costs
-// beside them), the fewest among equals.
-int choose_splits(int tiles, int kblocks, int slots) {
-    int best = 1;
-    double best_cost = -1.0;
-    for (int s = 1; s <= MAX_CLUSTER && s <= kblocks; ++s) {
-        const double cost = ((long long)tiles * s + slots - 1) / slots * ((kblocks + s - 1) / s + 4.0 + (s > 1 ? 2.0 : 0.0));
-        if (best_cost < 0 || cost < best_cost - 1e-9) { best = s; best_cost = cost; }
+// The tile (16, 32, 64 or 128 tokens beside 128 features; 256: pairs) and the parts of K.  Rounds of the CTAs over the device's places
+// times (blocks of K of each + what a CTA costs beside them); the fewest parts among equals.
+void choose(int M, int N, int K, int sms, int* tile, int* splits) {
+    const int kblocks = (K + BK - 1) / BK;
+    if (*tile == 0) {
+        *tile = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+        if (M > 128 && (long long)((M + 255) / 256) * ((N + 255) / 256) >= sms / 2) *tile = 256;
     }
-    return best;
+    if (*tile == 256) { *splits = 1; return; }
+    const long long tiles = (long long)((N + BM - 1) / BM) * ((M + *tile - 1) / *tile);
+    const int slots = sms * (*tile <= 64 ? 2 : 1);
+    double best = -1.0;
+    *splits = 1;
+    for (int s = 1; s <= MAX_SPLITS && s <= kblocks; ++s) {
+        const double cost = (double)((tiles * s + slots - 1) / slots) * ((kblocks + s - 1) / s + 6.0) + (s > 1 ? 6.0 : 0.0);
+        if (best < 0 || cost < best - 1e-9) { *splits = s; best = cost; }
+    }
 }
 
 }  // namespace
 
-// out [M, N] (float32 or bfloat16) = x times w transposed, with scales (above); xs [M, ceil(K / 128)], ws [ceil(N / 128), ceil(K / 128)].
-// kind: 0 chooses the tile; 16, 32, 64: swapped, that many tokens on the narrow side; 128: plain, 128 x 128; 256: plain, 256 x 256 on
-// pairs of CTAs.  splits: 0 chooses, or the CTAs (1 to 8) that share a tile's K (1 on pairs).  early_w: w and ws are not results of a kernel that may still run when this one starts, and the first tiles of w may
-// be read before the kernel in front has ended.  error_flag: where a wait that ran out leaves its number (null: see ph_fp8_take_error).
-PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int M, int N, int K, int kind,
-                          int splits, int early_w, int* error_flag, cudaStream_t stream) {
+// How ph_gemm_fp8 would cut an M x N x K product on the current device, where *tile and *splits are 0: the tile, and the parts of K.
+PH_EXPORT int ph_gemm_fp8_plan(int M, int N, int K, int* tile, int* splits) {
+    if (M < 1 || N < 1 || K < 1 || !tile || !splits) return fail(PH_ERR_ARG, "gemm_fp8: no plan for M %d, N %d, K %d", M, N, K);
+    if (*splits == 0) choose(M, N, K, multiprocessors(), tile, splits);
+    else {
+        int whole = 0;
+        choose(M, N, K, multiprocessors(), tile, &whole);
+    }
+    return PH_OK;
+}
+
+// out = x times w transposed, with scales (above); xs [M, ceil(K / 128)], ws [ceil(N / 128), ceil(K / 128)].  tile: 16, 32, 64 or 128 tokens
+// beside 128 features, or 256: 256 x 256 on pairs of CTAs (one part).  splits: parts of K, 1 to 16.  With several, parts is room for
+// [splits][M, N] float32: the sums of each part go there, and then, where out is given, their sum to out.  With one, or for the sum,
+// out [M, N] is float32 or bfloat16.  early_w: w and ws are not results of a kernel that may still run when this one starts, and the first
+// tiles of w may be read before the kernel in front has ended.  error_flag: where a wait that ran out leaves its number (null: see
+// ph_fp8_take_error).
+PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const float* ws, void* out, int out_dtype, int M, int N, int K, int tile,
+                          int splits, float* parts, int early_w, int* error_flag, cudaStream_t stream) {
     if (M == 0) return PH_OK;
-    if (!x || !xs || !w || !ws || !out || M < 1 || N < 1 || K < 1 || !valid_dtype(out_dtype) || splits < 0 || splits > MAX_CLUSTER)
-        return fail(PH_ERR_ARG, "gemm_fp8: bad arguments (M %d, N %d, K %d, splits %d)", M, N, K, splits);
+    if (!x || !xs || !w || !ws || M < 1 || N < 1 || K < 1 || !valid_dtype(out_dtype)) return fail(PH_ERR_ARG, "gemm_fp8: bad arguments (M %d, N %d, K %d)", M, N, K);
     if (K % 16) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: K = %d must be a multiple of 16 (16-byte rows for TMA)", K);
     if (((uintptr_t)x | (uintptr_t)w) & 15) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: operands must be 16-byte aligned");
     Params p = {};
-    p.xs = xs; p.ws = ws; p.out = out; p.out_bf16 = out_dtype == PH_BF16; p.M = M; p.N = N; p.kblocks = (K + BK - 1) / BK;
-    p.early_w = early_w; p.error_flag = error_flag;
-    if (splits > p.kblocks) return fail(PH_ERR_ARG, "gemm_fp8: %d splits for %d blocks of K", splits, p.kblocks);
-    if (kind == 0) {
-        kind = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-        if (M > 128 && (long long)((M + 255) / 256) * ((N + 255) / 256) >= multiprocessors() / 2 && splits == 0) kind = 256;
+    p.xs = xs; p.ws = ws; p.M = M; p.N = N; p.kblocks = (K + BK - 1) / BK; p.splits = splits; p.early_w = early_w; p.error_flag = error_flag;
+    if (splits < 1 || splits > MAX_SPLITS || splits > p.kblocks) return fail(PH_ERR_ARG, "gemm_fp8: %d parts of K for %d blocks (at most %d)", splits, p.kblocks, MAX_SPLITS);
+    if (splits == 1 ? !out : !parts) return fail(PH_ERR_ARG, "gemm_fp8: no room for the result");
+    if (splits > 1 && out && ((uintptr_t)parts & 15)) return fail(PH_ERR_ARG, "gemm_fp8: parts that are summed here must be 16-byte aligned");
+    p.out = splits > 1 ? parts : out;
+    p.out_bf16 = out_dtype == PH_BF16;
+    int rc;
+    switch (tile) {
+        case 16: rc = launch<16>(x, w, p, K, stream); break;
+        case 32: rc = launch<32>(x, w, p, K, stream); break;
+        case 64: rc = launch<64>(x, w, p, K, stream); break;
+        case 128: rc = launch<128>(x, w, p, K, stream); break;
+        case 256:
+            if (splits > 1) return fail(PH_ERR_ARG, "gemm_fp8: pairs of CTAs keep K whole");
+            return launch_pair(x, w, p, K, stream);
+        default: return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 128, 256", tile);
     }
-    if (kind == 256) {
-        if (splits > 1) return fail(PH_ERR_ARG, "gemm_fp8: pairs of CTAs keep K whole");
-        p.splits = 1;
-        return launch_pair(x, w, p, K, stream);
-    }
-    const int narrow = kind == 128 ? N : M;
-    const int tiles = (int)std::min<long long>((long long)(((kind == 128 ? M : N) + BM - 1) / BM) * ((narrow + kind - 1) / kind), 1 << 24);
-    p.splits = splits ? splits : choose_splits(tiles, p.kblocks, multiprocessors() * (kind <= 64 ? 2 : 1));
-    switch (kind) {
-        case 16: return launch<16, true>(x, w, p, K, stream);
-        case 32: return launch<32, true>(x, w, p, K, stream);
-        case 64: return launch<64, true>(x, w, p, K, stream);
-        case 128: return launch<128, false>(x, w, p, K, stream);
-        default: return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 128, 256", kind);
-    }
+    if (rc != PH_OK || splits == 1 || !out) return rc;
+    const long long values = (long long)M * N, grid = (values + 1023) / 1024;
+    if (grid > 0x7fffffffLL) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: %d x %d is too much", M, N);
+    if (p.out_bf16) launch_overlapped(sum_parts_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)parts, splits, values, (__nv_bfloat16*)out);
+    else launch_overlapped(sum_parts_kernel<float>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)parts, splits, values, (float*)out);
+    return check_launch("gemm_fp8 (sum of the parts)");
 }
 
 // The number that a wait which ran out has left on the current device since the last call (0: none); waits for the device.

@@ -242,7 +242,7 @@ def test_product(M, N, K, out):
     fp8.check_errors()
 
 
-@pytest.mark.parametrize("tile,splits", [(t, s) for t in (16, 32, 64, 128) for s in (1, 2, 3, 5, 8)] + [(256, 1)])
+@pytest.mark.parametrize("tile,splits", [(t, s) for t in (16, 32, 64, 128) for s in (1, 2, 3, 7, 16)] + [(256, 1)])
 @pytest.mark.parametrize("M,N", [(1, 200), (40, 200), (150, 200), (290, 515)])
 def test_product_of_every_tile_and_split(M, N, splits, tile):
     """Small whole numbers and scales that are powers of two: every sum is exact in float32, so every variant gives the same bits."""
@@ -253,12 +253,33 @@ def test_product_of_every_tile_and_split(M, N, splits, tile):
     w = torch.randint(-4, 5, (N, K), generator=g, device=DEV).float().to(torch.float8_e4m3fn)
     xs = torch.exp2(torch.randint(-2, 3, (M, kblocks(K)), generator=g, device=DEV).float())
     ws = torch.exp2(torch.randint(-2, 3, (kblocks(N), kblocks(K)), generator=g, device=DEV).float())
-    held = torch.full((M + 2, N), -7.0, device=DEV)
-    fp8.gemm(x, xs, w, ws, held[1:M + 1], tile=tile, splits=splits)
     want = (x.double() * spread(xs.double(), 1, M, K)) @ (w.double() * spread(ws.double(), 128, N, K)).T
-    assert torch.equal(held[1:M + 1].double(), want)
-    assert (held[0] == -7).all() and (held[M + 1] == -7).all()
+    held = torch.full((splits + 2, M, N), -7.0, device=DEV)
+    if splits > 1:
+        fp8.gemm(x, xs, w, ws, held[1:splits + 1], tile=tile, splits=splits)
+        assert torch.equal(held[1:splits + 1].double().sum(0), want)
+    else:
+        fp8.gemm(x, xs, w, ws, held[1], tile=tile, splits=1)
+        assert torch.equal(held[1].double(), want)
+    assert (held[0] == -7).all() and (held[splits + 1] == -7).all()
+    for dtype in DT.values():
+        assert torch.equal(fp8.gemm(x, xs, w, ws, out_dtype=dtype, tile=tile), want.to(dtype))
     fp8.check_errors()
+
+
+def test_product_into_places_off_their_boundaries():
+    """Outputs that start on their own type's boundary only, at widths whose rows would allow vectors."""
+    from purhie_b200.csrc import fp8
+    for M, N, K, tile in ((3, 260, 1040, 16), (70, 132, 2064, 64), (300, 264, 400, 256)):
+        x, xs, w, ws = operands(M, N, K, M)
+        for dtype in DT.values():
+            held = torch.zeros(M * N + 9, dtype=dtype, device=DEV)
+            y = held[1:M * N + 1].view(M, N)
+            for splits in (0, 1):
+                y.fill_(float("nan"))
+                fp8.gemm(x, xs, w, ws, y, tile=tile, splits=splits)
+                check_product(y, x, xs, w, ws)
+            assert held[0] == 0 and (held[M * N + 1:] == 0).all()
 
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
@@ -277,10 +298,9 @@ def test_product_refusals():
     x, xs, w, ws = operands(4, 64, 144, 1)
     with pytest.raises(KernelError, match="multiple of 16"):
         fp8.gemm(x[:, :136].contiguous(), xs, w[:, :136].contiguous(), ws)
-    with pytest.raises(KernelError, match="splits"):
-        fp8.gemm(x, xs, w, ws, splits=3)
-    with pytest.raises(KernelError, match="splits"):
-        fp8.gemm(x, xs, w, ws, splits=9)
+    for splits in (3, 17, -1):
+        with pytest.raises(KernelError, match="parts of K"):
+            fp8.gemm(x, xs, w, ws, splits=splits)
     with pytest.raises(KernelError, match="pairs"):
         fp8.gemm(x, xs, w, ws, tile=256, splits=2)
     with pytest.raises(KernelError, match="tile"):
