@@ -143,7 +143,8 @@ template <int BN> struct Tile {
     static constexpr int STAGES = (CTAS_PER_SM == 2 ? 96 : 192) * 1024 / STAGE_BYTES;
     static constexpr int BUFFERS = BN >= 64 ? 4 : 128 / BN;              // accumulators in tensor memory
     static constexpr int TMEM_COLS = BUFFERS * BN;
-    static constexpr int FACTORS_BYTES = FACTOR_BLOCKS * BN * 4;
+    static constexpr int FACTORS_LD = BN + 4;                            // (lanes write down a column: on eight banks, not on one)
+    static constexpr int FACTORS_BYTES = FACTOR_BLOCKS * FACTORS_LD * 4;
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + FACTORS_BYTES + 256;
     static constexpr int CHUNK = BN >= 64 ? 32 : 16;                     // columns of an accumulator that are read at a time
     static_assert(TMEM_COLS * CTAS_PER_SM <= 512, "tensor memory");
@@ -245,14 +246,16 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             const int some = min(FACTOR_BLOCKS, kb1 - base);
             if (base > kb0) asm volatile("bar.sync 1, 128;" ::: "memory");
             if (lane < some) {
+                float v[BN / 4];
+#pragma unroll
+                for (int i = 0; i < BN / 4; ++i) v[i] = p.xs[(size_t)min(m0 + warp - 2 + 4 * i, p.M - 1) * p.kblocks + base + lane];
                 const float s = ws[base + lane];
-#pragma unroll 8
-                for (int token = warp - 2; token < BN; token += 4)
-                    factors[lane * BN + token] = p.xs[(size_t)min(m0 + token, p.M - 1) * p.kblocks + base + lane] * s;
+#pragma unroll
+                for (int i = 0; i < BN / 4; ++i) factors[lane * Cfg::FACTORS_LD + warp - 2 + 4 * i] = v[i] * s;
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             for (int b = 0; b < some; ++b) {
-                const float4* f = (const float4*)(factors + b * BN);
+                const float4* f = (const float4*)(factors + b * Cfg::FACTORS_LD);
                 ok = ok && wait(&acc_full[buf], buf_phase, flag, PH_ERR_FP8_EPILOGUE);
                 __syncwarp();
                 tc_fence_after();
