@@ -285,7 +285,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             }
         }
         // the lanes of a warp hold neighbouring features of a token: whole lines leave straight from the registers
-        if (p.out_bf16 && splits == 1) {
+        if (p.out_bf16) {
             // (two tokens at a time: the even lanes store a pair of features of the one, the odd lanes of the other)
             const int odd = lane & 1, pair = n - odd;
             const bool wide = (p.N & 1) == 0 && ((uintptr_t)p.out & 3) == 0;
@@ -399,8 +399,9 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
 }
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c_inner, int c_row) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(c_inner), "r"(c_row) : "memory");
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int c_inner, int c_row, int c_part) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(c_inner), "r"(c_row), "r"(c_part)
+                 : "memory");
 }
 // a += v * f on two values at once.
 __device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t v0, uint32_t v1, float f) {
@@ -449,7 +450,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int a_tiles = p.a_tiles, b_tiles = (p.N + PAIR_BN - 1) / PAIR_BN;
-    const int tiles = a_tiles * b_tiles, first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+    const int splits = p.splits, items = a_tiles * b_tiles * splits, first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+    // item i: part i % splits of the K of tile i / splits
+    auto part_of_k = [&](int i, int& kb0, int& kb1) {
+        kb0 = (int)((long long)p.kblocks * (i % splits) / splits);
+        kb1 = (int)((long long)p.kblocks * (i % splits + 1) / splits);
+    };
 
     pdl_launch_dependents();
     if (warp < 4) {
@@ -458,9 +464,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int t = first; t < tiles && ok; t += stride) {
+            for (int i = first; i < items && ok; i += stride) {
+                const int t = i / splits;
+                int kb0, kb1;
+                part_of_k(i, kb0, kb1);
                 const int a0 = (t % a_tiles) * 2 * BM + (int)rank * BM, b0 = (t / a_tiles) * PAIR_BN + (int)rank * PAIR_HALF;
-                for (int kb = 0; kb < p.kblocks; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) { ok = false; break; }
                     const uint32_t bar = cluster_addr(&full[stage], 0);
                     // The leader alone announces the bytes of both; the peer's may land first (the count of bytes owed may run
@@ -480,8 +489,10 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             int stage = 0, buf = 0;
             uint32_t phase = 0, buf_phase = 0;
             bool ok = true;
-            for (int t = first; t < tiles && ok; t += stride) {
-                for (int kb = 0; kb < p.kblocks; ++kb) {
+            for (int i = first; i < items && ok; i += stride) {
+                int kb0, kb1;
+                part_of_k(i, kb0, kb1);
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!wait(&full[stage], phase, flag, PH_ERR_FP8_MMA) || !wait(&acc_empty[buf], buf_phase ^ 1, flag, PH_ERR_FP8_MMA)) { ok = false; break; }
                     tc_fence_after();
                     const uint64_t adesc = smem_desc(smem_a + stage * A_BYTES), bdesc = smem_desc(smem_b + stage * PAIR_HALF * BK);
@@ -497,17 +508,20 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         } else if (warp >= 2) {
             // Two warps look the scales up, four blocks of K at a time and some groups ahead, and leave their products in shared memory:
             // 2048 x 9472 x 4096 takes 79 us, and 87 where the epilogue's threads load them for themselves, however far ahead.
-            const int i = threadIdx.x - 64;
+            const int r = threadIdx.x - 64;
             int g = 0;
             uint32_t g_phase = 0;
             bool ok = true;
-            for (int t = first; t < tiles && ok; t += stride) {
-                const int row = (t % a_tiles) * 2 * BM + (int)rank * BM + i, nb = (t / a_tiles) * 2;
+            for (int i = first; i < items && ok; i += stride) {
+                const int t = i / splits;
+                int kb0, kb1;
+                part_of_k(i, kb0, kb1);
+                const int row = (t % a_tiles) * 2 * BM + (int)rank * BM + r, nb = (t / a_tiles) * 2;
                 const float* x0 = p.xs + (size_t)min(row, p.M - 1) * p.kblocks;
                 const float* x1 = p.xs + (size_t)min(row + 64, p.M - 1) * p.kblocks;
                 const float* w0 = p.ws + (size_t)nb * p.kblocks;
                 const float* w1 = p.ws + (size_t)min(nb + 1, (p.N - 1) / BK) * p.kblocks;
-                for (int kb = 0; kb < p.kblocks; kb += 4) {
+                for (int kb = kb0; kb < kb1; kb += 4) {
                     float a[4], b[4], u[4], v[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -516,7 +530,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     }
                     ok = wait(&fac_empty[g], g_phase ^ 1, flag, PH_ERR_FP8_EPILOGUE);
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                    float* f = factors + g * 2 * 4 * BM + i;
+                    float* f = factors + g * 2 * 4 * BM + r;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         f[j * BM] = a[j] * u[j]; f[j * BM + 64] = b[j] * u[j];
@@ -540,11 +554,11 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         uint32_t g_phase = 0;
         const uint32_t give_0 = cluster_addr(&acc_empty[0], 0), give_1 = cluster_addr(&acc_empty[1], 0);
         uint32_t taddr = 0;
-        // this thread's factor of block kb (each block of a tile once, in order)
-        auto next_factor = [&](int kb) {
-            if ((kb & 3) == 0) ok = ok && wait(&fac_full[group], g_phase, flag, PH_ERR_FP8_EPILOGUE);
-            const float f = factors[((group * 2 + half) * 4 + (kb & 3)) * BM + q * 32 + lane];
-            if ((kb & 3) == 3 || kb + 1 == p.kblocks) {
+        // this thread's factor of the item's block number b of `blocks` (each once, in order)
+        auto next_factor = [&](int b, int blocks) {
+            if ((b & 3) == 0) ok = ok && wait(&fac_full[group], g_phase, flag, PH_ERR_FP8_EPILOGUE);
+            const float f = factors[((group * 2 + half) * 4 + (b & 3)) * BM + q * 32 + lane];
+            if ((b & 3) == 3 || b + 1 == blocks) {
                 __syncwarp();
                 if (lane == 0) arrive(&fac_empty[group]);
                 if (++group == PAIR_GROUPS) { group = 0; g_phase ^= 1; }
@@ -559,7 +573,11 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * PAIR_BN + half * PAIR_HALF);
             tmem_ld32(taddr, r);
         };
-        for (int t = first; t < tiles; t += stride) {
+        for (int i = first; i < items; i += stride) {
+            const int t = i / splits;
+            int blocks, kb0;
+            part_of_k(i, kb0, blocks);
+            blocks -= kb0;
             const int row0 = (t % a_tiles) * 2 * BM + (int)rank * BM + q * 32, n0 = (t / a_tiles) * PAIR_BN + half * PAIR_HALF;
             const int row = row0 + lane;
             float acc[PAIR_HALF];
@@ -567,22 +585,22 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             for (int j = 0; j < PAIR_HALF; ++j) acc[j] = 0.0f;
             // The loads run one chunk of 32 columns ahead of the multiply-adds, over the end of a block too, and so does the factor.
             uint32_t r[2][32];
-            float f = next_factor(0), f_next = 0.0f;
+            float f = next_factor(0, blocks), f_next = 0.0f;
             next_accumulator(r[0]);
 #pragma unroll 1
-            for (int kb = 0; kb < p.kblocks; ++kb) {
+            for (int b = 0; b < blocks; ++b) {
 #pragma unroll
                 for (int c = 0; c < PAIR_HALF / 32; ++c) {
                     tmem_ld_wait();
                     if (c + 1 < PAIR_HALF / 32) {
                         tmem_ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
-                        if (c == 1 && kb + 1 < p.kblocks) f_next = next_factor(kb + 1);
+                        if (c == 1 && b + 1 < blocks) f_next = next_factor(b + 1, blocks);
                     } else {
                         tc_fence_before();                            // all of it is in registers: the accumulator is free
                         __syncwarp();
                         if (lane == 0) arrive_cluster(buf ? give_1 : give_0);
                         if (++buf == 2) { buf = 0; buf_phase ^= 1; }
-                        if (kb + 1 < p.kblocks) next_accumulator(r[0]);
+                        if (b + 1 < blocks) next_accumulator(r[0]);
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) fma2(acc[c * 32 + j], acc[c * 32 + j + 1], r[c & 1][j], r[c & 1][j + 1], f);
@@ -616,12 +634,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     __syncwarp();
                     const int col = n0 + b * (p.tma_store == 1 ? 64 : 32);
                     if (lane == 0) {
-                        if (col < p.N) tma_store_2d(&map_out, box, col, row0);
+                        if (col < p.N) tma_store_3d(&map_out, box, col, row0, i % splits);
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");       // one group a box, stored or not: the count above goes by them
                     }
                 }
             } else if (row < p.M) {
-                const size_t at = (size_t)row * p.N + n0;
+                const size_t at = ((size_t)(i % splits) * p.M + row) * p.N + n0;
 #pragma unroll
                 for (int j = 0; j < PAIR_HALF; ++j)
                     if (n0 + j < p.N) {
@@ -668,16 +686,16 @@ bool make_map(CUtensorMap* out, const void* ptr, int rows, int K, int box_rows) 
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// out [rows, cols] seen as boxes of 32 rows x 128 bytes, 128-byte swizzle.
-bool make_out_map(CUtensorMap* out, const void* ptr, bool bf16, int rows, int cols) {
+// out [parts, rows, cols] seen as boxes of 32 rows x 128 bytes, 128-byte swizzle.
+bool make_out_map(CUtensorMap* out, const void* ptr, bool bf16, int parts, int rows, int cols) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     const int size = bf16 ? 2 : 4;
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)cols * size};
-    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), 32};
-    const cuuint32_t elem[2] = {1, 1};
-    return fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)parts};
+    const cuuint64_t strides[2] = {(cuuint64_t)cols * size, (cuuint64_t)rows * cols * size};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / size), 32, 1};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    return fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(ptr), dims, strides, box, elem,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -689,9 +707,9 @@ int launch_pair(const void* x, const void* w, Params p, int K, cudaStream_t stre
     // the copy engine stores where its rules allow: rows of a multiple of 16 bytes on 16-byte boundaries
     mo = ma;
     p.tma_store = 0;
-    if ((p.N * (p.out_bf16 ? 2LL : 4LL)) % 16 == 0 && ((uintptr_t)p.out & 15) == 0 && make_out_map(&mo, p.out, p.out_bf16, p.M, p.N)) p.tma_store = p.out_bf16 ? 1 : 2;
+    if ((p.N * (p.out_bf16 ? 2LL : 4LL)) % 16 == 0 && ((uintptr_t)p.out & 15) == 0 && make_out_map(&mo, p.out, p.out_bf16, p.splits, p.M, p.N)) p.tma_store = p.out_bf16 ? 1 : 2;
     p.a_tiles = (p.M + 2 * BM - 1) / (2 * BM);
-    const long long tiles = (long long)p.a_tiles * ((p.N + PAIR_BN - 1) / PAIR_BN);
+    const long long tiles = (long long)p.a_tiles * ((p.N + PAIR_BN - 1) / PAIR_BN) * p.splits;
     if (tiles > 0x3fffffffLL) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8_pair: %d x %d has too many tiles", p.M, p.N);
     const int clusters = (int)std::min<long long>(tiles, multiprocessors() / 2);
     cudaLaunchConfig_t cfg = {};
@@ -755,7 +773,7 @@ PH_EXPORT int ph_gemm_fp8_plan(int M, int N, int K, int* tile, int* splits) {
 }
 
 // out = x times w transposed, with scales (above); xs [M, ceil(K / 128)], ws [ceil(N / 128), ceil(K / 128)].  tile: 16, 32, 64 or 128 tokens
-// beside 128 features, or 256: 256 x 256 on pairs of CTAs (one part).  splits: parts of K, 1 to 16.  With several, parts is room for
+// beside 128 features, or 256: 256 x 256 on pairs of CTAs.  splits: parts of K, 1 to 16.  With several, parts is room for
 // [splits][M, N] float32: the sums of each part go there, and then, where out is given, their sum to out.  With one, or for the sum,
 // out [M, N] is float32 or bfloat16.  early_w: w and ws are not results of a kernel that may still run when this one starts, and the first
 // tiles of w may be read before the kernel in front has ended.  error_flag: where a wait that ran out leaves its number (null: see
@@ -772,7 +790,7 @@ PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const f
     if (splits == 1 ? !out : !parts) return fail(PH_ERR_ARG, "gemm_fp8: no room for the result");
     if (splits > 1 && out && ((uintptr_t)parts & 15)) return fail(PH_ERR_ARG, "gemm_fp8: parts that are summed here must be 16-byte aligned");
     p.out = splits > 1 ? parts : out;
-    p.out_bf16 = out_dtype == PH_BF16;
+    p.out_bf16 = splits == 1 && out_dtype == PH_BF16;
     int rc;
     switch (tile) {
         case 16: rc = launch<16>(x, w, p, K, stream); break;
@@ -780,14 +798,14 @@ PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const f
         case 64: rc = launch<64>(x, w, p, K, stream); break;
         case 128: rc = launch<128>(x, w, p, K, stream); break;
         case 256:
-            if (splits > 1) return fail(PH_ERR_ARG, "gemm_fp8: pairs of CTAs keep K whole");
-            return launch_pair(x, w, p, K, stream);
+            rc = launch_pair(x, w, p, K, stream);
+            break;
         default: return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 128, 256", tile);
     }
     if (rc != PH_OK || splits == 1 || !out) return rc;
     const long long values = (long long)M * N, grid = (values + 1023) / 1024;
     if (grid > 0x7fffffffLL) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: %d x %d is too much", M, N);
-    if (p.out_bf16) launch_overlapped(sum_parts_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)parts, splits, values, (__nv_bfloat16*)out);
+    if (out_dtype == PH_BF16) launch_overlapped(sum_parts_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)parts, splits, values, (__nv_bfloat16*)out);
     else launch_overlapped(sum_parts_kernel<float>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)parts, splits, values, (float*)out);
     return check_launch("gemm_fp8 (sum of the parts)");
 }
