@@ -29,7 +29,7 @@ register_signatures("fp8", {
     "ph_fp8_take_error": [c_void_p],
     "ph_gemm_fp8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
                     c_void_p],
-    "ph_gemm_fp8_plan": [c_int, c_int, c_int, c_void_p, c_void_p],
+    "ph_gemm_fp8_plan": [c_int, c_int, c_int, c_int, c_void_p, c_void_p],
 })
 
 BLOCK = 128
@@ -172,9 +172,10 @@ def check_errors() -> None:
 
 @functools.lru_cache(maxsize=4096)
 def plan(M: int, N: int, K: int, device: int = 0, tile: int = 0, splits: int = 0) -> Tuple[int, int]:
-    """How a product is cut on the current device (number ``device``) where ``tile`` and ``splits`` are 0: tokens of a tile, parts of K."""
+    """How a whole product is cut on the current device (number ``device``) where ``tile`` or ``splits`` is 0: tokens of a tile, parts
+    of K."""
     t, s = c_int(tile), c_int(splits)
-    call("fp8", "ph_gemm_fp8_plan", M, N, K, ctypes.addressof(t), ctypes.addressof(s))
+    call("fp8", "ph_gemm_fp8_plan", M, N, K, 1, ctypes.addressof(t), ctypes.addressof(s))
     return t.value, s.value
 
 
@@ -184,7 +185,7 @@ def gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: tor
     [ceil(N / 128), ceil(K / 128)], K a multiple of 16, sums in float32, out float32 or bfloat16 (``out_dtype`` where out is not
     given).  ``splits`` > 1: K is cut into that many parts and out is [splits, M, N] float32, the sums of each, for a consumer that
     adds them up (``add_rmsnorm``, ``gated``); 0: cut as the kernel likes it, and out is the whole sum.  ``tile`` (0: the kernel's own
-    choice): 16, 32, 64 or 128 tokens beside 128 features, or 256 x 256 on pairs of CTAs.  ``early_w``: w is not the result of a
+    choice): 16, 32 or 64 tokens beside 128 features, or 256 x 256 on pairs of CTAs.  ``early_w``: w is not the result of a
     kernel that may still run when the product starts (a model's weight), so its first tiles may be read before the kernel in
     front has ended."""
     M, K = _matrix("gemm_fp8", "x", x)
@@ -206,6 +207,8 @@ def gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: tor
     out = x.new_empty(shape, dtype=dtype) if out is None else _check("gemm_fp8", "out", out, shape, dtype)
     if not M:
         return out
+    if tile < 0 or splits < 0:
+        raise KernelError(f"gemm_fp8: tile {tile} and splits {splits} must not be negative")
     if not tile or not splits:
         tile, splits = plan(M, N, K, x.get_device(), tile, splits)
     parts = out if parted else x.new_empty((splits, M, N), dtype=F32) if splits > 1 else None
