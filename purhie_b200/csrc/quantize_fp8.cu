@@ -13,6 +13,7 @@
 // memory: each input is read once and held in registers until its block's scale is known.
 // The reference's counterpart is its 8-bit activation blocks (src/matvec_q.hip), whose scales are per 32 values.
 #include "common.cuh"
+#include "shared_limit.cuh"
 
 #include <cuda_fp8.h>
 
@@ -52,29 +53,72 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // The place of a lane's value i inside its block.
 template <bool VEC> __device__ __forceinline__ int place(int lane16, int i) { return VEC ? lane16 * 8 + i : lane16 + 16 * i; }
 
+// A lane's eight values of a block as they lie in memory, and what is asked of them: a bfloat16 block waits for its scale in
+// half the registers, and its largest magnitude is found two values at a time.
+template <typename T> struct Held;
+template <> struct Held<float> {
+    float v[8];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    }
+    __device__ __forceinline__ void load(const float* p) { load8(p, v); }
+    __device__ __forceinline__ void set(int i, float x) { v[i] = x; }
+    __device__ __forceinline__ float get(int i) const { return v[i]; }
+    __device__ __forceinline__ float largest() const {
+        float m = fabsf(v[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
+        return m;
+    }
+};
+template <> struct Held<__nv_bfloat16> {
+    uint32_t v[4];
+    __device__ __forceinline__ void clear() { v[0] = v[1] = v[2] = v[3] = 0; }
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+    }
+    __device__ __forceinline__ void set(int i, __nv_bfloat16 x) {
+        const uint32_t bits = __bfloat16_as_ushort(x);
+        v[i >> 1] = (i & 1) ? (v[i >> 1] & 0xffffu) | bits << 16 : (v[i >> 1] & 0xffff0000u) | bits;
+    }
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float((i & 1) ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16); }
+    __device__ __forceinline__ float largest() const {
+        __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v[0]));
+#pragma unroll
+        for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v[i])));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+};
+
 // A lane's eight values of the block that starts at column k0 of a row of K (zeros behind the row's end).
 template <bool VEC, typename T>
-__device__ __forceinline__ void load_block(const T* row, int k0, int lane16, int K, float* v) {
+__device__ __forceinline__ void hold_block(const T* row, int k0, int lane16, int K, Held<T>& h) {
+    h.clear();
     if (VEC) {
-        if (k0 + lane16 * 8 < K) load8(row + k0 + lane16 * 8, v);
-        else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        }
+        if (k0 + lane16 * 8 < K) h.load(row + k0 + lane16 * 8);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int k = k0 + place<false>(lane16, i);
-            v[i] = k < K ? to_float<T>(row[k]) : 0.0f;
+            if (k < K) h.set(i, row[k]);
         }
     }
 }
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_block(const T* row, int k0, int lane16, int K, float* v) {
+    Held<T> h;
+    hold_block<VEC>(row, k0, lane16, K, h);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = h.get(i);
+}
 
-template <bool VEC>
-__device__ __forceinline__ void store_block(uint8_t* row, int k0, int lane16, int K, const float* v, float inverse) {
+template <bool VEC, typename V>
+__device__ __forceinline__ void store_block(uint8_t* row, int k0, int lane16, int K, const V& v, float inverse) {
     uint32_t p[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = pack2(v[2 * i] * inverse, v[2 * i + 1] * inverse);
+    for (int i = 0; i < 4; ++i) p[i] = pack2(v.get(2 * i) * inverse, v.get(2 * i + 1) * inverse);
     if (VEC) {
         if (k0 + lane16 * 8 < K) *(uint2*)(row + k0 + lane16 * 8) = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
     } else {
@@ -86,13 +130,10 @@ __device__ __forceinline__ void store_block(uint8_t* row, int k0, int lane16, in
     }
 }
 
-// A lane's share of a block is in v: the block's scale to *scale, its values to q.  Every lane of the warp calls this.
-template <bool VEC>
-__device__ __forceinline__ void finish_block(uint8_t* row, float* scale, bool live, int k0, int lane16, int K, const float* v) {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
-    const float a = max_nan(half_warp_max(m), LEAST);
+// A lane's share of a block: the block's scale to *scale, its values to the row.  Every lane of the warp calls this.
+template <bool VEC, typename V>
+__device__ __forceinline__ void finish_block(uint8_t* row, float* scale, bool live, int k0, int lane16, int K, const V& v) {
+    const float a = max_nan(half_warp_max(v.largest()), LEAST);
     if (!live) return;
     if (lane16 == 0) *scale = a / TOP;
     store_block<VEC>(row, k0, lane16, K, v, TOP / a);
@@ -100,27 +141,29 @@ __device__ __forceinline__ void finish_block(uint8_t* row, float* scale, bool li
 
 constexpr int ROW_THREADS = 256;
 
-// U blocks of a row (or of several rows) for each half warp, all of them asked for before the first is worked on.
+// U neighbouring blocks of rows for each half warp, all of them asked for before the first is worked on.
 template <typename T, bool VEC, int U>
-__global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __restrict__ x, long long stride, uint8_t* __restrict__ q, float* __restrict__ scales, long long blocks,
-                                     int kblocks, int K) {
+__global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __restrict__ x, long long stride, uint8_t* __restrict__ q, float* __restrict__ scales, unsigned blocks,
+                                     unsigned kblocks, int K) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane16 = threadIdx.x & 15;
-    const long long first = ((long long)blockIdx.x * (ROW_THREADS / 16) + (threadIdx.x >> 4)) * U;
-    float v[U][8];
-    long long row[U];
+    const unsigned first = (blockIdx.x * (ROW_THREADS / 16) + (threadIdx.x >> 4)) * U;
+    unsigned row = first / kblocks, b = first - row * kblocks;
+    Held<T> v[U];
+    unsigned at_row[U];
     int k0[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const long long b = first + u < blocks ? first + u : blocks - 1;
-        row[u] = b / kblocks;
-        k0[u] = (int)(b - row[u] * kblocks) * BLOCK;
-        load_block<VEC>(x + row[u] * stride, k0[u], lane16, K, v[u]);
+        at_row[u] = row;
+        k0[u] = (int)b * BLOCK;
+        if (first + u < blocks) hold_block<VEC>(x + row * stride, k0[u], lane16, K, v[u]);
+        else v[u].clear();
+        if (++b == kblocks) { b = 0; ++row; }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        finish_block<VEC>(q + row[u] * K, scales + first + u, first + u < blocks, k0[u], lane16, K, v[u]);
+        finish_block<VEC>(q + (size_t)at_row[u] * K, scales + first + u, first + u < blocks, k0[u], lane16, K, v[u]);
 }
 
 // One CTA for each 128 x 128 block of a weight: 16 half warps, eight rows each.
@@ -131,17 +174,16 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
     const int lane16 = threadIdx.x & 15, half = threadIdx.x >> 4;
     const int k0 = blockIdx.x * BLOCK;
     const long long t0 = (long long)blockIdx.y * BLOCK;
-    float v[8][8];
+    Held<T> v[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
         const long long t = t0 + r * 16 + half;
-        load_block<VEC>(x + (t < T_rows ? t : 0) * stride, k0, lane16, t < T_rows ? K : 0, v[r]);
+        if (t < T_rows) hold_block<VEC>(x + t * stride, k0, lane16, K, v[r]);
+        else v[r].clear();
     }
-    float m = 0.0f;
+    float m = v[0].largest();
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[r][i]));
+    for (int r = 1; r < 8; ++r) m = max_nan(m, v[r].largest());
     m = half_warp_max(m);
     m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 16));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
@@ -224,9 +266,10 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(NormParams p) 
         const int b = half + u * halves;
         float w[8];
         load_block<VEC>(p.weight, b * BLOCK, lane16, p.E, w);
+        Held<float> y;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] = v[u][i] * f * w[i];
-        finish_block<VEC>(p.q + r * p.E, p.scales + r * p.kblocks + b, b < p.kblocks, b * BLOCK, lane16, p.E, v[u]);
+        for (int i = 0; i < 8; ++i) y.v[i] = v[u][i] * f * w[i];
+        finish_block<VEC>(p.q + r * p.E, p.scales + r * p.kblocks + b, b < p.kblocks, b * BLOCK, lane16, p.E, y);
     }
 }
 
@@ -245,47 +288,90 @@ __device__ __forceinline__ float gated_value(const Gate& gate, float g, float u)
     return __fdividef(g, 1.0f + __expf(-gate.alpha * g)) * (u + gate.shift);
 }
 
-// Rows of (g0, u0, g1, u1, ...), in `parts` parts that are summed first, to gated rows of F in 8 bits.
-template <typename T, bool VEC>
+// Rows of (g0, u0, g1, u1, ...), in `parts` parts that are summed first, to gated rows of F in 8 bits; U blocks for each half warp.
+template <typename T, bool VEC, int U>
 __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restrict__ gate_up, int parts, long long part_stride, uint8_t* __restrict__ q, float* __restrict__ scales,
-                                 long long blocks, int kblocks, int F, Gate gate) {
+                                 unsigned blocks, unsigned kblocks, int F, Gate gate) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane16 = threadIdx.x & 15;
-    const long long b = (long long)blockIdx.x * (ROW_THREADS / 16) + (threadIdx.x >> 4);
-    const long long at = b < blocks ? b : blocks - 1;
-    const long long row = at / kblocks;
-    const int k0 = (int)(at - row * kblocks) * BLOCK;
-    const T* src = gate_up + row * 2 * F;
-    float h[8];
-    if (VEC) {
-        float g[16];
+    const unsigned first = (blockIdx.x * (ROW_THREADS / 16) + (threadIdx.x >> 4)) * U;
+    unsigned row = first / kblocks, b = first - row * kblocks;
+    if (VEC && parts == 1) {
+        // one part: what is read waits as it lies in memory
+        Held<T> v[U][2];
+        unsigned at_row[U];
+        int k0[U];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) g[i] = 0.0f;
-        if (k0 + lane16 * 8 < F) {
-            for (int s = 0; s < parts; ++s) {
-                float a[16];
-                load8(src + s * part_stride + 2 * (k0 + lane16 * 8), a);
-                load8(src + s * part_stride + 2 * (k0 + lane16 * 8) + 8, a + 8);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) g[i] = s == 0 ? a[i] : g[i] + a[i];
+        for (int u = 0; u < U; ++u) {
+            at_row[u] = row;
+            k0[u] = (int)b * BLOCK;
+            v[u][0].clear();
+            v[u][1].clear();
+            if (first + u < blocks && k0[u] + lane16 * 8 < F) {
+                const T* src = gate_up + (size_t)row * 2 * F + 2 * (k0[u] + lane16 * 8);
+                v[u][0].load(src);
+                v[u][1].load(src + 8);
             }
+            if (++b == kblocks) { b = 0; ++row; }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = gated_value(gate, g[2 * i], g[2 * i + 1]);
-    } else {
+        for (int u = 0; u < U; ++u) {
+            Held<float> h;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int k = k0 + place<false>(lane16, i);
-            float g = 0.0f, u = 0.0f;
-            if (k < F) {
-                g = to_float<T>(src[2 * k]); u = to_float<T>(src[2 * k + 1]);
-                for (int s = 1; s < parts; ++s) { g += to_float<T>(src[s * part_stride + 2 * k]); u += to_float<T>(src[s * part_stride + 2 * k + 1]); }
-            }
-            h[i] = gated_value(gate, g, u);
+            for (int i = 0; i < 8; ++i) h.v[i] = gated_value(gate, v[u][i >> 2].get(2 * (i & 3)), v[u][i >> 2].get(2 * (i & 3) + 1));
+            finish_block<VEC>(q + (size_t)at_row[u] * F, scales + first + u, first + u < blocks, k0[u], lane16, F, h);
         }
+        return;
     }
-    finish_block<VEC>(q + row * F, scales + b, b < blocks, k0, lane16, F, h);
+#pragma unroll 1
+    for (int u = 0; u < U; ++u) {
+        const int k0 = (int)b * BLOCK;
+        const bool live = first + u < blocks;
+        const T* src = gate_up + (size_t)row * 2 * F;
+        Held<float> h;
+        if (VEC) {
+            float g[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) g[i] = 0.0f;
+            if (live && k0 + lane16 * 8 < F) {
+                for (int s = 0; s < parts; ++s) {
+                    float a[16];
+                    load8(src + s * part_stride + 2 * (k0 + lane16 * 8), a);
+                    load8(src + s * part_stride + 2 * (k0 + lane16 * 8) + 8, a + 8);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) g[i] = s == 0 ? a[i] : g[i] + a[i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h.v[i] = gated_value(gate, g[2 * i], g[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int k = k0 + place<false>(lane16, i);
+                float g = 0.0f, x = 0.0f;
+                if (live && k < F) {
+                    g = to_float<T>(src[2 * (size_t)k]); x = to_float<T>(src[2 * (size_t)k + 1]);
+                    for (int s = 1; s < parts; ++s) { g += to_float<T>(src[s * part_stride + 2 * (size_t)k]); x += to_float<T>(src[s * part_stride + 2 * (size_t)k + 1]); }
+                }
+                h.v[i] = gated_value(gate, g, x);
+            }
+        }
+        finish_block<VEC>(q + (size_t)row * F, scales + first + u, live, k0, lane16, F, h);
+        if (++b == kblocks) { b = 0; ++row; }
+    }
+}
+
+// The number of blocks and of CTAs for them; U blocks a half warp where that leaves every SM its fill of threads, else one.
+// (2,048 rows of 12,288 bfloat16 gated values: 37 us with one, whose index arithmetic and short waits add up.)
+constexpr int MANY = 4;
+inline bool count_blocks(long long rows, int width, unsigned* blocks, int* u, unsigned* ctas) {
+    const long long n = rows * ((width + BLOCK - 1) / BLOCK);
+    if (n > 0x7fffffffLL - 4 * ROW_THREADS) return false;
+    *blocks = (unsigned)n;
+    *u = n >= (long long)multiprocessors() * 8 * (ROW_THREADS / 16) * MANY ? MANY : 1;
+    *ctas = (unsigned)((n + (ROW_THREADS / 16) * *u - 1) / ((ROW_THREADS / 16) * *u));
+    return true;
 }
 
 inline bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
@@ -324,12 +410,13 @@ PH_EXPORT int ph_quantize_fp8(const void* x, int dtype, long long stride, void* 
         });
         return check_launch("quantize_fp8");
     }
-    const long long blocks = (long long)T * kblocks;
-    const long long grid = (blocks + ROW_THREADS / 16 - 1) / (ROW_THREADS / 16);
-    if (grid > 0x7fffffffLL) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: %lld blocks are too many", blocks);
+    unsigned blocks, ctas;
+    int u;
+    if (!count_blocks(T, K, &blocks, &u, &ctas)) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: %d x %d are too many blocks", T, K);
     PH_DISPATCH(dtype, X, {
-        if (vec) launch_overlapped(quantize_rows_kernel<X, true, 1>, dim3((unsigned)grid), dim3(ROW_THREADS), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, blocks, kblocks, K);
-        else launch_overlapped(quantize_rows_kernel<X, false, 1>, dim3((unsigned)grid), dim3(ROW_THREADS), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, blocks, kblocks, K);
+        auto kernel = vec ? (u == 1 ? quantize_rows_kernel<X, true, 1> : quantize_rows_kernel<X, true, MANY>)
+                          : (u == 1 ? quantize_rows_kernel<X, false, 1> : quantize_rows_kernel<X, false, MANY>);
+        launch_overlapped(kernel, dim3(ctas), dim3(ROW_THREADS), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, blocks, (unsigned)kblocks, K);
     });
     return check_launch("quantize_fp8");
 }
@@ -360,12 +447,14 @@ PH_EXPORT int ph_gated_fp8(const void* gate_up, int dtype, int parts, long long 
     if (gate) g = Gate{(int)gate[3], gate[0], gate[1], gate[2]};
     if (g.kind < 0 || g.kind > 2) return fail(PH_ERR_ARG, "gated_fp8: gate %d is not known", g.kind);
     const int kblocks = (F + BLOCK - 1) / BLOCK, size = dtype == PH_F32 ? 4 : 2;
-    const long long blocks = (long long)T * kblocks, grid = (blocks + ROW_THREADS / 16 - 1) / (ROW_THREADS / 16);
-    if (grid > 0x7fffffffLL) return fail(PH_ERR_UNSUPPORTED, "gated_fp8: %lld blocks are too many", blocks);
+    unsigned blocks, ctas;
+    int u;
+    if (!count_blocks(T, F, &blocks, &u, &ctas)) return fail(PH_ERR_UNSUPPORTED, "gated_fp8: %d x %d are too many blocks", T, F);
     const bool vec = F % 8 == 0 && aligned(gate_up, 16) && aligned(q, 8) && (part_stride * size) % 16 == 0;
     PH_DISPATCH(dtype, X, {
-        if (vec) launch_overlapped(gated_fp8_kernel<X, true>, dim3((unsigned)grid), dim3(ROW_THREADS), 0, stream, (const X*)gate_up, parts, part_stride, (uint8_t*)q, scales, blocks, kblocks, F, g);
-        else launch_overlapped(gated_fp8_kernel<X, false>, dim3((unsigned)grid), dim3(ROW_THREADS), 0, stream, (const X*)gate_up, parts, part_stride, (uint8_t*)q, scales, blocks, kblocks, F, g);
+        auto kernel = vec ? (u == 1 ? gated_fp8_kernel<X, true, 1> : gated_fp8_kernel<X, true, MANY>)
+                          : (u == 1 ? gated_fp8_kernel<X, false, 1> : gated_fp8_kernel<X, false, MANY>);
+        launch_overlapped(kernel, dim3(ctas), dim3(ROW_THREADS), 0, stream, (const X*)gate_up, parts, part_stride, (uint8_t*)q, scales, blocks, (unsigned)kblocks, F, g);
     });
     return check_launch("gated_fp8");
 }
