@@ -216,8 +216,8 @@ struct NormParams {
     float* scales;
 };
 
-template <typename A, bool VEC, int U, int THREADS>
-__global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(NormParams p) {
+template <typename A, bool VEC, int U>
+__global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(NormParams p) {
     __shared__ float scratch[32];
     const int lane16 = threadIdx.x & 15, half = threadIdx.x >> 4, halves = blockDim.x >> 4;
     pdl_launch_dependents();
@@ -362,14 +362,16 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
     }
 }
 
-// The number of blocks and of CTAs for them; U blocks a half warp where that leaves every SM its fill of threads, else one.
-// (2,048 rows of 12,288 bfloat16 gated values: 37 us with one, whose index arithmetic and short waits add up.)
-constexpr int MANY = 4;
-inline bool count_blocks(long long rows, int width, unsigned* blocks, int* u, unsigned* ctas) {
+// Blocks for each half warp where they are many: what a lane holds while it waits is the same for both types.
+template <typename T> constexpr int MANY = 8 / (int)sizeof(T);
+
+// The number of blocks and of CTAs for them.  Several blocks a half warp once every SM has twice its fill of threads, else one: 2,048
+// rows of 12,288 gated bfloat16 values take 24.0 us with four, 29.9 with one and 34.7 with eight; 256 such rows 6.5 and 5.5.
+inline bool count_blocks(long long rows, int width, int many, unsigned* blocks, int* u, unsigned* ctas) {
     const long long n = rows * ((width + BLOCK - 1) / BLOCK);
     if (n > 0x7fffffffLL - 4 * ROW_THREADS) return false;
     *blocks = (unsigned)n;
-    *u = n >= (long long)multiprocessors() * 8 * (ROW_THREADS / 16) * MANY ? MANY : 1;
+    *u = n >= (long long)multiprocessors() * 16 * (ROW_THREADS / 16) ? many : 1;
     *ctas = (unsigned)((n + (ROW_THREADS / 16) * *u - 1) / ((ROW_THREADS / 16) * *u));
     return true;
 }
@@ -378,15 +380,15 @@ inline bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1))
 
 template <typename A, bool VEC>
 int launch_norm(const NormParams& p, int n, cudaStream_t stream) {
-    // blocks per half warp: as few as a CTA of 512 threads allows where rows are few, so that a row is spread wide
-    const int u = p.kblocks <= 32 ? 1 : p.kblocks <= 64 ? 2 : p.kblocks <= 128 ? 4 : 8;
+    // blocks per half warp: as few as a CTA of 1,024 threads allows, so that a row is spread wide and waits for its sum the
+    // shortest (2,048 rows of 5,120: 20.5 us with one, 24.5 with two, 29.8 with four)
+    const int u = p.kblocks <= 64 ? 1 : p.kblocks <= 128 ? 2 : 4;
     const int halves = (p.kblocks + u - 1) / u;
     const int threads = (halves * 16 + 31) / 32 * 32;
     switch (u) {
-        case 1: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 1, 512>, dim3(n), dim3(threads), 0, stream, p); break;
-        case 2: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 2, 512>, dim3(n), dim3(threads), 0, stream, p); break;
-        case 4: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 4, 512>, dim3(n), dim3(threads), 0, stream, p); break;
-        default: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 8, 512>, dim3(n), dim3(threads), 0, stream, p); break;
+        case 1: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 1>, dim3(n), dim3(threads), 0, stream, p); break;
+        case 2: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 2>, dim3(n), dim3(threads), 0, stream, p); break;
+        default: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 4>, dim3(n), dim3(threads), 0, stream, p); break;
     }
     return check_launch("add_rmsnorm_fp8");
 }
@@ -410,12 +412,13 @@ PH_EXPORT int ph_quantize_fp8(const void* x, int dtype, long long stride, void* 
         });
         return check_launch("quantize_fp8");
     }
+    const int many = dtype == PH_F32 ? MANY<float> : MANY<__nv_bfloat16>;
     unsigned blocks, ctas;
     int u;
-    if (!count_blocks(T, K, &blocks, &u, &ctas)) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: %d x %d are too many blocks", T, K);
+    if (!count_blocks(T, K, many, &blocks, &u, &ctas)) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: %d x %d are too many blocks", T, K);
     PH_DISPATCH(dtype, X, {
-        auto kernel = vec ? (u == 1 ? quantize_rows_kernel<X, true, 1> : quantize_rows_kernel<X, true, MANY>)
-                          : (u == 1 ? quantize_rows_kernel<X, false, 1> : quantize_rows_kernel<X, false, MANY>);
+        auto kernel = vec ? (u == 1 ? quantize_rows_kernel<X, true, 1> : quantize_rows_kernel<X, true, MANY<X>>)
+                          : (u == 1 ? quantize_rows_kernel<X, false, 1> : quantize_rows_kernel<X, false, MANY<X>>);
         launch_overlapped(kernel, dim3(ctas), dim3(ROW_THREADS), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, blocks, (unsigned)kblocks, K);
     });
     return check_launch("quantize_fp8");
@@ -447,13 +450,14 @@ PH_EXPORT int ph_gated_fp8(const void* gate_up, int dtype, int parts, long long 
     if (gate) g = Gate{(int)gate[3], gate[0], gate[1], gate[2]};
     if (g.kind < 0 || g.kind > 2) return fail(PH_ERR_ARG, "gated_fp8: gate %d is not known", g.kind);
     const int kblocks = (F + BLOCK - 1) / BLOCK, size = dtype == PH_F32 ? 4 : 2;
+    const int many = dtype == PH_F32 ? MANY<float> : MANY<__nv_bfloat16>;
     unsigned blocks, ctas;
     int u;
-    if (!count_blocks(T, F, &blocks, &u, &ctas)) return fail(PH_ERR_UNSUPPORTED, "gated_fp8: %d x %d are too many blocks", T, F);
+    if (!count_blocks(T, F, many, &blocks, &u, &ctas)) return fail(PH_ERR_UNSUPPORTED, "gated_fp8: %d x %d are too many blocks", T, F);
     const bool vec = F % 8 == 0 && aligned(gate_up, 16) && aligned(q, 8) && (part_stride * size) % 16 == 0;
     PH_DISPATCH(dtype, X, {
-        auto kernel = vec ? (u == 1 ? gated_fp8_kernel<X, true, 1> : gated_fp8_kernel<X, true, MANY>)
-                          : (u == 1 ? gated_fp8_kernel<X, false, 1> : gated_fp8_kernel<X, false, MANY>);
+        auto kernel = vec ? (u == 1 ? gated_fp8_kernel<X, true, 1> : gated_fp8_kernel<X, true, MANY<X>>)
+                          : (u == 1 ? gated_fp8_kernel<X, false, 1> : gated_fp8_kernel<X, false, MANY<X>>);
         launch_overlapped(kernel, dim3(ctas), dim3(ROW_THREADS), 0, stream, (const X*)gate_up, parts, part_stride, (uint8_t*)q, scales, blocks, (unsigned)kblocks, F, g);
     });
     return check_launch("gated_fp8");
