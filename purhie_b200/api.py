@@ -319,7 +319,10 @@ class Model:
 
 
 def load_model(path: str, dtype: str = "bfloat16", options: Optional[dict] = None) -> Model:
-    """``inference_load_model``: read config.json and the safetensors of ``path`` onto the device."""
+    """``inference_load_model``: read config.json and the safetensors of ``path`` onto the device.  ``options``: kernel choices of
+    the parts, {"gemm": "auto" | "tcgen05" | "simple" | "fp8", "attention": "auto" | "flash" | "generic"}; "fp8" holds the matrices
+    of attention and feed-forwards in 8 bits (``inference.h``)."""
+    native.ensure_libraries_for_options(options)
     h = native.lib().inference_load_model_ex(str(path).encode(), dtype.encode(), json.dumps(options or {}).encode())
     if not h:
         raise native.last_error()
@@ -331,6 +334,7 @@ def load_model_random(config, seed: int, dtype: str = "bfloat16", std: float = 0
     """A model of ``config`` (a typed configuration, a dict or config.json text) with seeded random weights made on
     the device: the values :func:`purhie_b200.weights.write_random_model` stores for the same seed."""
     from .weights import _config_json
+    native.ensure_libraries_for_options(options)
     h = native.lib().inference_load_model_random_ex(_config_json(config), int(seed), dtype.encode(), float(std),
                                                     float(scale_low), float(scale_high), json.dumps(options or {}).encode())
     if not h:

@@ -67,7 +67,11 @@ void sampler_reset(sampler_t* s);
 /* A folder with config.json and model.safetensors (or a shard index); bfloat16 compute.  NULL on failure. */
 inference_model_t* inference_load_model(const char* model_dir);
 /* dtype: "bfloat16" or "float32" (a true 32-bit path: float32 weights, activations, cache and products).
- * options_json: NULL or {"gemm": "auto|tcgen05|simple", "attention": "auto|flash|generic"}. */
+ * options_json: NULL or {"gemm": "auto|tcgen05|simple|fp8", "attention": "auto|flash|generic"}.  "fp8" (bfloat16 models): the
+ * matrices of the attention parts and of the feed-forwards that are not routed are brought to 8 bits when they are loaded
+ * (e4m3, a scale for each block of 128 x 128), their rows in every step (a scale for each 128 values), and multiplied that way;
+ * the embedding, the output matrix and every other part stay as they are.  Half the memory and twice the decode rate of the
+ * matrices concerned, at 8 bits' precision. */
 inference_model_t* inference_load_model_ex(const char* model_dir, const char* dtype, const char* options_json);
 /* Seeded random weights made on the device for the configuration in config_json (the text of a config.json):
  * matrices N(0, 0.02), norm weights 1.  The values are those inference_write_random_model stores. */

@@ -171,11 +171,11 @@ def check_errors() -> None:
 
 
 @functools.lru_cache(maxsize=4096)
-def plan(M: int, N: int, K: int, device: int = 0, tile: int = 0, splits: int = 0) -> Tuple[int, int]:
-    """How a whole product is cut on the current device (number ``device``) where ``tile`` or ``splits`` is 0: tokens of a tile, parts
-    of K."""
+def plan(M: int, N: int, K: int, device: int = 0, tile: int = 0, splits: int = 0, whole: bool = True) -> Tuple[int, int]:
+    """How a product is cut on the current device (number ``device``) where ``tile`` or ``splits`` is 0: tokens of a tile, parts of
+    K.  ``whole``: the whole sum is wanted, not the parts."""
     t, s = c_int(tile), c_int(splits)
-    call("fp8", "ph_gemm_fp8_plan", M, N, K, 1, ctypes.addressof(t), ctypes.addressof(s))
+    call("fp8", "ph_gemm_fp8_plan", M, N, K, int(whole), ctypes.addressof(t), ctypes.addressof(s))
     return t.value, s.value
 
 

@@ -83,6 +83,7 @@ class Engine:
     @staticmethod
     def load_handle(model_dir: str, dtype: str = "bfloat16", options: Optional[dict] = None):
         L = native.lib()
+        native.ensure_libraries_for_options(options)
         h = L.inference_load_model_ex(str(model_dir).encode(), dtype.encode(), json.dumps(options or {}).encode())
         if not h:
             raise native.last_error()
@@ -93,6 +94,7 @@ class Engine:
                       scale_high: float = 1.0, options: Optional[dict] = None):
         from ..weights import _config_json
         L = native.lib()
+        native.ensure_libraries_for_options(options)
         h = L.inference_load_model_random_ex(_config_json(config), int(seed), dtype.encode(), float(std), float(scale_low),
                                              float(scale_high), json.dumps(options or {}).encode())
         if not h:

@@ -26,6 +26,7 @@ const char* kGemmErrors[] = {"the TMA producer waited too long for a free stage"
 std::string flag_text(int which, int code) {
     if (which == 0) {
         const char* t = (code >= 101 && code <= 103) ? kGemmErrors[code - 101] : "error";
+        if (code >= 131 && code <= 133) return "gemm_fp8: " + std::string(kGemmErrors[code - 131]) + " (status " + std::to_string(code) + ")";
         return "gemm_tcgen05: " + std::string(t) + " (status " + std::to_string(code) + ")";
     }
     const char* t = code == 111 ? "the attention producer waited too long for a free stage"

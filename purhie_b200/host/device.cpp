@@ -109,7 +109,8 @@ FlashKernels g_flash{};
 GemmKernels g_gemm{};
 LatentKernels g_latent{};
 LayersKernels g_layers{};
-bool g_core_ok = false, g_flash_ok = false, g_gemm_ok = false, g_latent_ok = false, g_layers_ok = false;
+Fp8Kernels g_fp8{};
+bool g_fp8_ok = false, g_core_ok = false, g_flash_ok = false, g_gemm_ok = false, g_latent_ok = false, g_layers_ok = false;
 
 std::string own_dir() {
     Dl_info info;
@@ -293,12 +294,28 @@ const LayersKernels& layers_kernels() {
     return g_layers;
 }
 
+const Fp8Kernels& fp8_kernels() {
+    if (g_fp8_ok) return g_fp8;
+    std::lock_guard<std::mutex> lock(g_lib_mutex);
+    if (g_fp8_ok) return g_fp8;
+    void* h = open_library("fp8");
+    bind(h, "fp8", "ph_quantize_fp8", g_fp8.quantize);
+    bind(h, "fp8", "ph_add_rmsnorm_fp8", g_fp8.add_rmsnorm);
+    bind(h, "fp8", "ph_gated_fp8", g_fp8.gated);
+    bind(h, "fp8", "ph_gemm_fp8_plan", g_fp8.plan);
+    bind(h, "fp8", "ph_gemm_fp8", g_fp8.gemm);
+    bind(h, "fp8", "ph_fp8_last_error", g_fp8.last_error);
+    g_fp8_ok = true;
+    return g_fp8;
+}
+
 void require_library(const std::string& name) {
     if (name == "core") core_kernels();
     else if (name == "flash") flash_kernels();
     else if (name == "gemm100") gemm_kernels();
     else if (name == "latent") latent_kernels();
     else if (name == "layers") layers_kernels();
+    else if (name == "fp8") fp8_kernels();
     else {
         std::lock_guard<std::mutex> lock(g_lib_mutex);
         open_library(name);

@@ -296,6 +296,17 @@ struct GemmKernels {
                         cudaStream_t);
     const char* (*last_error)(void);
 };
+// 8-bit linear layers (quantize_fp8.cu, gemm_fp8.cu): rows and weights in e4m3 with scales, the norm and the gated activation that
+// give such rows, the product
+struct Fp8Kernels {
+    int (*quantize)(const void*, int, long long, void*, float*, int, int, int, cudaStream_t);
+    int (*add_rmsnorm)(const float*, const void*, int, int, long long, const float*, float, const int32_t*, int, int, int, float*, void*, float*,
+                       cudaStream_t);
+    int (*gated)(const void*, int, int, long long, void*, float*, int, int, const float*, cudaStream_t);
+    int (*plan)(int, int, int, int, int*, int*);
+    int (*gemm)(const void*, const float*, const void*, const float*, void*, int, int, int, int, int, int, float*, int, int*, cudaStream_t);
+    const char* (*last_error)(void);
+};
 struct LayersKernels {
     int (*supports)(int, int, int, int, int, int, int, int, int);
     int (*shares)(int, int, int, int, int, int32_t*);
@@ -316,7 +327,8 @@ QE_API const FlashKernels& flash_kernels();
 QE_API const GemmKernels& gemm_kernels();
 QE_API const LatentKernels& latent_kernels();
 QE_API const LayersKernels& layers_kernels();
-QE_API void require_library(const std::string& name);      // "core", "flash", "gemm100", "latent", "layers": open it now
+QE_API const Fp8Kernels& fp8_kernels();
+QE_API void require_library(const std::string& name);      // "core", "flash", "gemm100", "latent", "layers", "fp8": open it now
 QE_API extern long long g_launches;                          // launcher calls so far (for the bench's count)
 
 // Time per kernel class, for finding out where a step's time goes (the reference prints such a breakdown under

@@ -284,6 +284,12 @@ def ensure_libraries_for(model_handle) -> None:
         build_library(name)
 
 
+def ensure_libraries_for_options(options) -> None:
+    """Compile the kernel libraries that loading a model with these options needs already."""
+    if (options or {}).get("gemm") == "fp8":
+        build_library("fp8")
+
+
 def profile_enabled() -> bool:
     return bool(lib().qe_profile_enabled())
 

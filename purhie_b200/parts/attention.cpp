@@ -246,9 +246,9 @@ public:
         }
         QE_CUDA(cudaStreamSynchronize(src.stream()));
         for (Tensor& t : parts) src.release(t);
-        qkv_proj_ = Linear(qkv, "qkv_proj", gemm_);
-        q_only_proj_ = Linear(qkv.rows(0, q_width_), "q_proj", gemm_);
-        o_proj_ = Linear(src.fetch(name_of("o_proj")), "o_proj", gemm_);
+        qkv_proj_ = Linear::bound(src, qkv, "qkv_proj", gemm_);
+        q_only_proj_ = qkv_proj_.first_features(q_width_, "q_proj", gemm_);
+        o_proj_ = Linear::bound(src, src.fetch(name_of("o_proj")), "o_proj", gemm_);
         auto constants = [&](const std::vector<float>& values) {
             Tensor t = src.arena().alloc(DType::F32, {(int64_t)values.size()});
             QE_CUDA(cudaMemcpyAsync(t.data, values.data(), values.size() * sizeof(float), cudaMemcpyHostToDevice, src.stream()));
@@ -274,6 +274,7 @@ public:
     std::vector<std::string> required_libraries() const override {
         std::vector<std::string> libs = {"core"};
         if (qkv_proj_.fast() || o_proj_.fast()) libs.push_back("gemm100");
+        if (qkv_proj_.eight_bit() || o_proj_.eight_bit()) libs.push_back("fp8");
         if (use_flash()) libs.push_back("flash");
         return libs;
     }
@@ -284,7 +285,8 @@ public:
     }
     std::vector<Part*> children() override { return position_ ? std::vector<Part*>{position_.get()} : std::vector<Part*>{}; }
     // rows per tile of the products for many tokens (the tcgen05 pair kernel): a scheduler may end a step there
-    int preferred_row_multiple() const override { return (qkv_proj_.fast() || o_proj_.fast()) ? 256 : 0; }
+    int preferred_row_multiple() const override { return (qkv_proj_.fast() || o_proj_.fast() || qkv_proj_.eight_bit() || o_proj_.eight_bit()) ? 256 : 0; }
+    bool takes_eight_bit_rows(const StepContext&) const override { return qkv_proj_.eight_bit(); }
 
     // how far back a row can look at most: the window, the mask's block, the smaller of the two (0: all the way)
     int reach() const { return window_ && chunk_ ? std::min(window_, chunk_) : window_ ? window_ : chunk_; }
@@ -635,8 +637,8 @@ public:
         }
         QE_CUDA(cudaStreamSynchronize(src.stream()));
         for (Tensor& t : parts) src.release(t);
-        in_proj_ = Linear(all, "qkvg_proj", gemm_);
-        o_proj_ = Linear(src.fetch(name_of("o_proj")), "o_proj", gemm_);
+        in_proj_ = Linear::bound(src, all, "qkvg_proj", gemm_);
+        o_proj_ = Linear::bound(src, src.fetch(name_of("o_proj")), "o_proj", gemm_);
         if (has_norm_) {
             q_norm_ = src.fetch(name_of("q_norm"));
             k_norm_ = src.fetch(name_of("k_norm"));
@@ -650,9 +652,13 @@ public:
     }
 
     std::vector<std::string> required_libraries() const override {
-        return (in_proj_.fast() || o_proj_.fast()) ? std::vector<std::string>{"core", "gemm100"} : std::vector<std::string>{"core"};
+        std::vector<std::string> libs = {"core"};
+        if (in_proj_.fast() || o_proj_.fast()) libs.push_back("gemm100");
+        if (in_proj_.eight_bit() || o_proj_.eight_bit()) libs.push_back("fp8");
+        return libs;
     }
-    int preferred_row_multiple() const override { return (in_proj_.fast() || o_proj_.fast()) ? 256 : 0; }
+    int preferred_row_multiple() const override { return (in_proj_.fast() || o_proj_.fast() || in_proj_.eight_bit() || o_proj_.eight_bit()) ? 256 : 0; }
+    bool takes_eight_bit_rows(const StepContext&) const override { return in_proj_.eight_bit(); }
     CacheNeed cache_need() const override { return CacheNeed::pages(kv_heads_, head_dim_, window_, value_dim_); }
 
     // bfloat16 with sizes the tensor-core kernel takes: a tile of 16 rows and all heads per CTA; else the plain kernel

@@ -62,14 +62,17 @@ public:
         const bool may_work_ahead = may_defer && ctx.option("norm_ahead") != "off";
         const bool ff_unscaled = ff_ && may_defer && ff_->takes_unscaled_rows(ctx);
         ctx.row_scale = RowScale();
-        Tensor xn = may_defer && mixer_->takes_unscaled_rows(ctx) ? mixer_norm_->forward_unscaled(stream, ctx, &ctx.row_scale)
-                                                                  : mixer_norm_->forward(stream, ctx);
+        // (a consumer whose first product is in 8 bits takes its rows from the norm that way)
+        Tensor xn = mixer_->takes_eight_bit_rows(ctx) ? mixer_norm_->forward_eight_bit(stream, ctx) : Tensor();
+        if (!xn.defined())
+            xn = may_defer && mixer_->takes_unscaled_rows(ctx) ? mixer_norm_->forward_unscaled(stream, ctx, &ctx.row_scale) : mixer_norm_->forward(stream, ctx);
         ctx.norm_ahead = may_work_ahead && ff_unscaled ? ff_norm_->offer(ctx) : (!ff_ && may_work_ahead) ? ctx.next_layer_norm : NormAhead();
         stream.add(mixer_->forward(xn, ctx, cache));
         stream.prepare(ctx.norm_ahead);
         ctx.row_scale = RowScale();
         if (!ff_) { ctx.norm_ahead = NormAhead(); return; }
-        xn = ff_unscaled ? ff_norm_->forward_unscaled(stream, ctx, &ctx.row_scale) : ff_norm_->forward(stream, ctx);
+        xn = ff_->takes_eight_bit_rows(ctx) ? ff_norm_->forward_eight_bit(stream, ctx) : Tensor();
+        if (!xn.defined()) xn = ff_unscaled ? ff_norm_->forward_unscaled(stream, ctx, &ctx.row_scale) : ff_norm_->forward(stream, ctx);
         ctx.norm_ahead = may_work_ahead ? ctx.next_layer_norm : NormAhead();
         stream.add(ff_->forward(xn, ctx));
         stream.prepare(ctx.norm_ahead);

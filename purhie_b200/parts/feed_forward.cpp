@@ -39,13 +39,17 @@ public:
         QE_CUDA(cudaStreamSynchronize(src.stream()));
         src.release(gate);
         src.release(up);
-        gate_up_ = Linear(both, "gate_up_proj", gemm_);
-        down_ = Linear(src.fetch(name_of("down_proj")), "down_proj", gemm_);
+        gate_up_ = Linear::bound(src, both, "gate_up_proj", gemm_);
+        down_ = Linear::bound(src, src.fetch(name_of("down_proj")), "down_proj", gemm_);
     }
 
     std::vector<std::string> required_libraries() const override {
-        return (gate_up_.fast() || down_.fast()) ? std::vector<std::string>{"core", "gemm100"} : std::vector<std::string>{"core"};
+        std::vector<std::string> libs = {"core"};
+        if (gate_up_.fast() || down_.fast()) libs.push_back("gemm100");
+        if (gate_up_.eight_bit() || down_.eight_bit()) libs.push_back("fp8");
+        return libs;
     }
+    bool takes_eight_bit_rows(const StepContext&) const override { return gate_up_.eight_bit(); }
 
     // bfloat16: the gate/up product's epilogue applies the norm's factor per row before the activation
     bool takes_unscaled_rows(const StepContext& ctx) const override {
@@ -68,7 +72,17 @@ public:
                              gate_.kind ? gate_constants : nullptr);
         Tensor act;
         if (gu.activated) act = gu.tensor;
-        else {
+        else if (down_.eight_bit()) {
+            // the activation gives the second product's rows in 8 bits
+            const Fp8Kernels& k = fp8_kernels();
+            act = ctx.workspace->get("ff_act8", {T, inter_}, DType::U8);
+            Tensor scales = ctx.workspace->get("ff_act8_scales", {T, (inter_ + 127) / 128}, DType::F32);
+            if (LaunchProfile::get().on())
+                LaunchProfile::get().note_cost((double)T * inter_ * (2.0 * gu.splits * dtype_size(gu.tensor.dtype) + 1.0), 0.0);
+            QE_LAUNCH(k, k.gated(gu.tensor.data, gu.tensor.code(), gu.splits, (long long)T * 2 * inter_, act.data, scales.as<float>(), T, (int)inter_,
+                                 gate_.kind ? gate_constants : nullptr, ctx.stream));
+            ctx.row8_scales = scales.as<float>();
+        } else {
             act = ctx.workspace->get("ff_act", {T, inter_}, compute_dtype);
             const CoreKernels& k = core_kernels();
             if (LaunchProfile::get().on())
@@ -102,12 +116,16 @@ public:
         return {{name_of("up_proj"), {inter_, hidden_}, Role::Matrix, Init::Normal}, {name_of("down_proj"), {hidden_, inter_}, Role::Matrix, Init::Normal}};
     }
     void bind(WeightSource& src) override {
-        up_ = Linear(src.fetch(name_of("up_proj")), "up_proj", gemm_);
-        down_ = Linear(src.fetch(name_of("down_proj")), "down_proj", gemm_);
+        up_ = Linear::bound(src, src.fetch(name_of("up_proj")), "up_proj", gemm_);
+        down_ = Linear::bound(src, src.fetch(name_of("down_proj")), "down_proj", gemm_);
     }
     std::vector<std::string> required_libraries() const override {
-        return (up_.fast() || down_.fast()) ? std::vector<std::string>{"core", "gemm100"} : std::vector<std::string>{"core"};
+        std::vector<std::string> libs = {"core"};
+        if (up_.fast() || down_.fast()) libs.push_back("gemm100");
+        if (up_.eight_bit() || down_.eight_bit()) libs.push_back("fp8");
+        return libs;
     }
+    bool takes_eight_bit_rows(const StepContext&) const override { return up_.eight_bit(); }
     Addend forward(const Tensor& x, StepContext& ctx) override {
         const int T = ctx.T;
         Addend u = up_(x, ctx, "mlp_up", compute_dtype, T, true);

@@ -4,6 +4,7 @@ namespace qe {
 
 namespace {
 constexpr int kBlockK = 64;
+constexpr int kScaleBlock = 128;          // 8 bits: values of K, and features, that share a scale
 inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Few tokens: the product is weight streaming.  The work items (128-feature tile, split of K) should fill whole
@@ -105,14 +106,65 @@ Linear::Linear(Tensor weight, std::string label, const std::string& gemm) : weig
     if (weight_.shape.size() != 2)
         throw ConfigError(label_ + ": a linear weight must be a matrix, got " + shape_text(weight_.shape));
     const bool takes = weight_.dtype == DType::BF16 && weight_.shape[1] % 8 == 0 && ((uintptr_t)weight_.data % 16) == 0;
-    if (weight_.dtype == DType::BF16 && (gemm == "auto" || gemm == "tcgen05")) {
+    if (weight_.dtype == DType::BF16 && (gemm == "auto" || gemm == "tcgen05" || gemm == "fp8")) {
         fast_ = takes;
         if (!takes && gemm == "tcgen05")
             throw KernelError(label_ + ": the tcgen05 kernel does not take a weight of shape " + shape_text(weight_.shape));
     }
 }
 
+Linear Linear::bound(WeightSource& src, Tensor weight, std::string label, const std::string& gemm) {
+    if (gemm != "fp8" || weight.dtype != DType::BF16 || weight.shape.size() != 2 || weight.shape[1] % 16) return Linear(std::move(weight), std::move(label), gemm);
+    const int N = (int)weight.shape[0], K = (int)weight.shape[1];
+    const Fp8Kernels& k = fp8_kernels();
+    Linear l;
+    l.label_ = std::move(label);
+    l.weight_ = src.arena().alloc(DType::U8, {N, K});
+    l.scales_ = src.arena().alloc(DType::F32, {ceil_div(N, kScaleBlock), ceil_div(K, kScaleBlock)});
+    QE_LAUNCH(k, k.quantize(weight.data, weight.code(), K, l.weight_.data, l.scales_.as<float>(), N, K, kScaleBlock, src.stream()));
+    QE_CUDA(cudaStreamSynchronize(src.stream()));
+    src.release(weight);
+    return l;
+}
+
+Linear Linear::first_features(int64_t n, std::string label, const std::string& gemm) const {
+    if (!eight_bit()) return Linear(weight_.rows(0, n), std::move(label), gemm);
+    Linear l = *this;
+    l.label_ = std::move(label);
+    l.weight_ = weight_.rows(0, n);
+    l.scales_ = scales_.rows(0, ceil_div(n, kScaleBlock));
+    return l;
+}
+
+Addend Linear::eight_bit_product(const Tensor& x, StepContext& ctx, const std::string& out_name, DType out_dtype, int M, bool allow_split, void* into) const {
+    const int N = (int)weight_.shape[0], K = (int)weight_.shape[1], kb = ceil_div(K, kScaleBlock);
+    const Fp8Kernels& k = fp8_kernels();
+    Workspace& ws = *ctx.workspace;
+    const void* rows = x.data;
+    const float* row_scales = ctx.row8_scales;
+    if (x.dtype != DType::U8) {
+        Tensor q = ws.get("linear_rows8", {M, K}, DType::U8), s = ws.get("linear_rows8_scales", {M, kb}, DType::F32);
+        if (LaunchProfile::get().on()) LaunchProfile::get().note_cost((double)M * K * (dtype_size(x.dtype) + 1) + 4.0 * M * kb, 0.0);
+        QE_LAUNCH(k, k.quantize(x.data, x.code(), K, q.data, s.as<float>(), M, K, 1, ctx.stream));
+        rows = q.data;
+        row_scales = s.as<float>();
+    }
+    if (!row_scales) throw Error(kInvalidState, label_ + ": rows in 8 bits came without their scales");
+    int tile = 0, splits = 0;
+    if (k.plan(M, N, K, allow_split ? 0 : 1, &tile, &splits) != 0) throw KernelError(k.last_error());
+    const bool hand_on = allow_split && splits > 1;          // whoever consumes the product adds the parts up
+    Tensor parts = splits > 1 ? ws.get(hand_on ? out_name + "_partial" : "linear_parts8", {splits, M, N}, DType::F32) : Tensor();
+    Tensor out;
+    if (!hand_on) out = into ? Tensor(into, out_dtype, {M, N}) : ws.get(out_name, {M, N}, out_dtype);
+    if (LaunchProfile::get().on())
+        LaunchProfile::get().note_cost((double)N * K + (double)M * K + (double)(hand_on ? parts.bytes() : out.bytes()), 2.0 * M * N * K);
+    QE_LAUNCH(k, k.gemm(rows, row_scales, weight_.data, scales_.as<float>(), hand_on ? nullptr : out.data, hand_on ? parts.code() : out.code(), M, N, K,
+                        tile, splits, splits > 1 ? parts.as<float>() : nullptr, 1, ctx.gemm_error, ctx.stream));
+    return hand_on ? Addend(parts, splits) : Addend(out, 1);
+}
+
 std::vector<std::string> Linear::required_libraries() const {
+    if (eight_bit()) return {"core", "fp8"};
     return fast_ ? std::vector<std::string>{"core", "gemm100"} : std::vector<std::string>{"core"};
 }
 
@@ -140,6 +192,10 @@ bool Linear::gives_partial_sums(int rows, bool allow_split) const {
 void Linear::into(const Tensor& x_in, StepContext& ctx, Tensor out, int rows) const {
     const int M = rows, N = (int)weight_.shape[0], K = (int)weight_.shape[1];
     if (M == 0) return;
+    if (eight_bit()) {
+        eight_bit_product(x_in, ctx, label_, out.dtype, M, false, out.data);
+        return;
+    }
     const CoreKernels& core = core_kernels();
     Tensor x = x_in;
     if (weight_.dtype == DType::F32 && x.dtype != DType::F32) {
@@ -167,6 +223,10 @@ Addend Linear::operator()(const Tensor& x_in, StepContext& ctx, const std::strin
                           bool allow_split, bool fuse_swiglu, float* add_into, const RowScale* scale, NormAhead* ahead,
                           const float* gate) const {
     const int M = rows, N = (int)weight_.shape[0], K = (int)weight_.shape[1];
+    if (eight_bit()) {
+        if (scale && scale->defined()) throw KernelError(label_ + ": rows without their factor reached a product in 8 bits");
+        return eight_bit_product(x_in, ctx, out_name, out_dtype, M, allow_split, nullptr);
+    }
     Workspace& ws = *ctx.workspace;
     const CoreKernels& core = core_kernels();
     Tensor x = x_in;

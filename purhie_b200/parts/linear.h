@@ -2,7 +2,8 @@
 //
 // float32 weights go through the exact-order CUDA-core kernel (the 32-bit path; also a 32-bit tensor met in a
 // bfloat16 model).  bfloat16 weights go through the tcgen05 tensor-core kernel when it takes the shape, else
-// through the plain kernel.  The reference picks a kernel by weight type and batch size the same way
+// through the plain kernel.  A weight held in 8 bits (bound(), option "gemm": "fp8") goes through the block-scaled product: its
+// rows come in 8 bits already, or are brought there first.  The reference picks a kernel by weight type and batch size the same way
 // (qmatvec_launch, src/qmatvec.cpp:274; matvec / matvec_multi, src/qwen_model.cpp:855-922).
 #pragma once
 
@@ -25,8 +26,14 @@ QE_API GemmPlan plan_gemm(int M, int N, int K, int sms, bool allow_split, bool f
 class QE_API Linear {
 public:
     Linear() = default;
-    // gemm: "auto" (tcgen05 where it takes the shape), "tcgen05" (demand it), "simple" (never)
+    // gemm: "auto" (tcgen05 where it takes the shape; "fp8" is the same here), "tcgen05" (demand it), "simple" (never)
     Linear(Tensor weight, std::string label, const std::string& gemm);
+    // As the constructor; with gemm "fp8" a bfloat16 weight of rows of a multiple of 16 values is brought to 8 bits (a scale for each
+    // block of 128 x 128) and given back to the source's arena.
+    static Linear bound(WeightSource& src, Tensor weight, std::string label, const std::string& gemm);
+    // The first n output features of a product in 8 bits, or of the weight.
+    Linear first_features(int64_t n, std::string label, const std::string& gemm) const;
+    bool eight_bit() const { return scales_.defined(); }
     bool defined() const { return weight_.defined(); }
     bool fast() const { return fast_; }
     int64_t out_features() const { return weight_.shape[0]; }
@@ -56,7 +63,10 @@ public:
     // Many rows, K cut into parts: float32 partial sums, linear in the rows, so whoever adds them up can apply the factor.
     bool gives_partial_sums(int rows, bool allow_split) const;
 private:
-    Tensor weight_;
+    // [M, N] in out_dtype, or (parts wanted and better) float32 parts of it
+    Addend eight_bit_product(const Tensor& x, StepContext& ctx, const std::string& out_name, DType out_dtype, int M, bool allow_split, void* out) const;
+    Tensor weight_;          // eight_bit(): bytes, e4m3
+    Tensor scales_;          // eight_bit(): float32 [ceil(N / 128), ceil(K / 128)]
     std::string label_;
     bool fast_ = false;
 };

@@ -17,6 +17,8 @@ DecoderModel::DecoderModel(ModelSpec spec, DType compute_dtype, Json options)
         if (layers_.back()->takes_lanes() != (spec_.residual_lanes > 0))
             throw ConfigError("layers of kind '" + layer.arrangement + "' do not fit a residual of " + std::to_string(spec_.residual_lanes) + " lanes");
     }
+    if (build_.options.get_string("gemm", "auto") == "fp8" && build_.compute_dtype != DType::BF16)
+        throw ConfigError("matrices in 8 bits (\"gemm\": \"fp8\") go with a bfloat16 model");
     final_norm_ = make_part_as<Norm>("norm", spec_.final_norm, build_);
     head_ = make_part_as<Head>("head", spec_.head, build_);
 }

@@ -175,6 +175,23 @@ public:
         return out;
     }
 
+    Tensor forward_eight_bit(ResidualStream& stream, StepContext& ctx) override {
+        constexpr int64_t kWidest = 32768;                            // that the kernel takes
+        if (size_ > kWidest) return Tensor();
+        if (stream.has_also || (stream.has_pending && stream.pending.transform.defined())) fold_all_addends(stream, ctx);
+        Tensor out = ctx.workspace->get("normed8", {ctx.T, size_}, DType::U8);
+        Tensor scales = ctx.workspace->get("normed8_scales", {ctx.T, (size_ + 127) / 128}, DType::F32);
+        const Fp8Kernels& k = fp8_kernels();
+        const Addend* pend = stream.has_pending ? &stream.pending : nullptr;
+        note_norm_cost(stream, ctx.T, size_, DType::U8, true);
+        QE_LAUNCH(k, k.add_rmsnorm(stream.x.as<float>(), pend ? pend->tensor.data : nullptr, pend ? pend->tensor.code() : 0, pend ? pend->splits : 1,
+                                   pend ? (long long)ctx.T * size_ : 0, weight_.as<float>(), (float)eps_, nullptr, ctx.T, ctx.T, (int)size_,
+                                   pend ? stream.x.as<float>() : nullptr, out.data, scales.as<float>(), ctx.stream));
+        stream.clear();
+        ctx.row8_scales = scales.as<float>();
+        return out;
+    }
+
     Tensor forward_lanes(ResidualStream& stream, StepContext& ctx, const float* in, const int32_t* rows, int n_rows) override {
         const int n = rows ? n_rows : ctx.T;
         Tensor out = ctx.workspace->get(rows ? "normed_rows" : "normed", {n, size_}, compute_dtype);

@@ -259,6 +259,7 @@ struct StepContext {
     int64_t residual_width = 0;
     int* gemm_error = nullptr;               // device words where kernels with bounded waits report giving up
     int* attention_error = nullptr;
+    const float* row8_scales = nullptr;      // of the rows that a part is handed in 8 bits (takes_eight_bit_rows), [T, ceil(E / 128)]
     RowScale row_scale;                      // set by an arrangement around a consumer that takes unscaled rows, else undefined
     NormAhead norm_ahead;                    // set by an arrangement around a part: the norm after the part's addition
     NormAhead next_layer_norm;               // set by the model around a layer: the first norm of the layer that runs next
@@ -345,7 +346,7 @@ class QE_API BuildContext {
 public:
     explicit BuildContext(DType compute = DType::F32, Json options = Json::object()) : compute_dtype(compute), options(std::move(options)) {}
     DType compute_dtype;
-    Json options;                            // "gemm": auto|tcgen05|simple, "attention": auto|flash|generic
+    Json options;                            // "gemm": auto|tcgen05|simple|fp8, "attention": auto|flash|generic
     // parts that several owners share (one rotary table for all layers): made once per key
     std::shared_ptr<Part> shared(const std::string& key, const std::function<std::shared_ptr<Part>()>& make);
 private:
@@ -396,6 +397,9 @@ public:
     virtual AddendTransform as_transform(float factor) const;
     // The norm's weight and eps, if it is x * rsqrt(mean(x^2) + eps) * weight over the row and nothing else.
     virtual bool plain_rms(const float** weight, float* eps) const { return false; }
+    // As forward() over all rows, in 8 bits: e4m3 values (a Tensor of bytes) with a scale for each 128 of a row, which goes to
+    // ctx.row8_scales.  A norm that has no such form does nothing and returns an undefined tensor.
+    virtual Tensor forward_eight_bit(ResidualStream&, StepContext&) { return Tensor(); }
     // The float32 rows x [n, width] normed in place (no addend, no cast): for an embedding that is normed before it
     // becomes the residual stream.  A norm that has no such form throws.
     virtual void apply_in_place(Tensor& x, StepContext& ctx, int n);
@@ -427,6 +431,8 @@ public:
     // leave the row's factor out (see RowScale).  A mixer that says nothing always gets finished rows.
     virtual bool takes_unscaled_rows(const StepContext&) const { return false; }
     virtual bool decode_layer(DecodeLayerSpec&) const { return false; }              // see DecodeLayerSpec
+    // True: forward() also takes x in 8 bits, with ctx.row8_scales (Norm::forward_eight_bit).
+    virtual bool takes_eight_bit_rows(const StepContext&) const { return false; }
 };
 
 class QE_API FeedForward : public Part {
@@ -435,6 +441,7 @@ public:
     virtual Addend forward(const Tensor& x, StepContext& ctx) = 0;
     virtual bool takes_unscaled_rows(const StepContext&) const { return false; }     // as Mixer's
     virtual bool decode_layer(DecodeLayerSpec&) const { return false; }
+    virtual bool takes_eight_bit_rows(const StepContext&) const { return false; }    // as Mixer's
 };
 
 class QE_API Embedding : public Part {
