@@ -296,6 +296,8 @@ def main():
     ap.add_argument("--page-size", type=int, default=16, help="tokens per cache page (the benchmark's configuration has 16)")
     ap.add_argument("--step-options", default="", metavar="JSON",
                     help="kernel choices of the step, for comparing two forms of it on one box, e.g. '{\"norm_ahead\": \"off\"}'")
+    ap.add_argument("--gemm", default="auto", choices=["auto", "fp8"],
+                    help="fp8: the layers' matrices in 8 bits with a scale for each 128 x 128, a workload of its own beside the headline")
     ap.add_argument("--design", default="", choices=["", "bozosun", "sizizen", "zerusun", "vokepel", "noditar", "defapel"],
                     help="instead of the headline workload: prefill and decode of this design at real layer sizes beside four "
                          "Qwen3 layers of equal size, with the time and roofline fraction of every kernel class")
@@ -321,7 +323,7 @@ def main():
         args.layers = shape["num_hidden_layers"]
     cfg = Qwen3Config.from_dict(dict(shape, num_hidden_layers=args.layers))
     pk = peaks()
-    model = load_model_random(cfg, SEED, "bfloat16", std=STD)
+    model = load_model_random(cfg, SEED, "bfloat16", std=STD, options={"gemm": args.gemm})
     max_batch = args.batch if args.phase != "all" else max(max(point_batches), args.batch)
     if args.phase != "all":
         args.no_points = True
@@ -371,7 +373,8 @@ def main():
         eng.add_request(i)
         eng.step([StepEntry(i, ids(PREFIX), [])])
 
-    weight_bytes = 2.0 * (cfg.num_hidden_layers * layer_mm + V * E)       # the embedding table is gathered, not streamed
+    matrix_bytes = 2.0 if args.gemm == "auto" else 1.0 + 4.0 / 128 / 128
+    weight_bytes = matrix_bytes * cfg.num_hidden_layers * layer_mm + 2.0 * V * E       # the embedding table is gathered, not streamed
     kv_bytes_per_token = 2.0 * 2 * cfg.num_hidden_layers * kvw
 
     def decode_run(batch, steps, warmup):
@@ -452,7 +455,7 @@ def main():
     out = {
         "metric": f"decode tok/s at batch {args.batch} from 2,048-token prefixes ({shape_name} shape)", "value": round(value, 1),
         "unit": "tokens/s", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup, "ms_per_step": round(ms_step, 4),
-        "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
+        "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "bf16" if args.gemm == "auto" else "e4m3 matrices, bf16", "data": "synthetic",
         "impl": "ours",
         "config": {"model": f"{shape_name} shape, random weights seed {SEED}", "global_batch": args.batch, "seq_len": PREFIX,
                    "context": CONTEXT, "parallelism": "single GPU", "layers": args.layers,

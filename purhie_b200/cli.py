@@ -26,7 +26,7 @@ import sys
 import time
 
 USAGE = ("Usage: qwen_demo <model_dir | --random CONFIG.json> \"<token ids>\" | @prompt_file [n_gen] [--temp T] [--top-k K] "
-         "[--top-p P] [--min-p P]\n       [--repeat-penalty R] [--seed S] [--ctx N] [--batch N] [--dtype bfloat16|float32] "
+         "[--top-p P] [--min-p P]\n       [--repeat-penalty R] [--seed S] [--ctx N] [--batch N] [--dtype bfloat16|float32] [--gemm auto|tcgen05|simple|fp8] "
          "[--tokens \"ids\"] [--tokens-file F]\n       [--random-prompt LEN] [--weights-seed S] [--block-size B] "
          "[--max-batch-tokens N] [--chunk N] [--ignore-eos]\n")
 _NOT_BUILT = {"--lm-head-q8": 0, "--draft": 1, "--drafts": 1, "--kv-q8": 0, "--kv-q4": 0, "--stage": 1}
@@ -52,7 +52,7 @@ def main(argv=None) -> int:
     sp = SamplerParams.defaults()
     sp.temperature = 0.0                      # greedy unless asked
     o = dict(n_gen=16, ctx=4096, batch=0, dtype="bfloat16", random_prompt=0, random=None, weights_seed=0, block=16,
-             budget=2048, chunk=512, ignore_eos=False, tokens=None, tokens_file=None)
+             budget=2048, chunk=512, ignore_eos=False, tokens=None, tokens_file=None, gemm="auto")
     positional = []
     i = 0
     while i < len(argv):
@@ -67,6 +67,7 @@ def main(argv=None) -> int:
         elif a == "--ctx": o["ctx"] = int(v); i += 1
         elif a == "--batch": o["batch"] = int(v); i += 1
         elif a == "--dtype": o["dtype"] = {"bf16": "bfloat16", "fp32": "float32"}.get(v, v); i += 1
+        elif a == "--gemm": o["gemm"] = v; i += 1
         elif a == "--random-prompt": o["random_prompt"] = int(v); i += 1
         elif a == "--random": o["random"] = v; i += 1
         elif a == "--weights-seed": o["weights_seed"] = int(v); i += 1
@@ -98,15 +99,18 @@ def main(argv=None) -> int:
     if not model_path and not o["random"]:
         sys.stdout.write(USAGE)
         return 1
+    if o["gemm"] not in ("auto", "tcgen05", "simple", "fp8"):
+        sys.stderr.write(f"qwen_demo: --gemm {o['gemm']} is not known\n{USAGE}")
+        return 1
     print(f"Sampling: temp {sp.temperature:g} top_k {sp.top_k} top_p {sp.top_p:g} min_p {sp.min_p:g} "
           f"repeat_penalty {sp.repeat_penalty:g} seed {sp.seed}")
     try:
         if o["random"]:
             with open(o["random"], "r", encoding="utf-8") as f:
                 config = json.load(f)
-            model = load_model_random(config, o["weights_seed"], dtype=o["dtype"])
+            model = load_model_random(config, o["weights_seed"], dtype=o["dtype"], options={"gemm": o["gemm"]})
         else:
-            model = load_model(model_path, dtype=o["dtype"])
+            model = load_model(model_path, dtype=o["dtype"], options={"gemm": o["gemm"]})
         # the prompts
         if o["random_prompt"] > 0:
             prompts = [uniform_ids(o["random_prompt"], model.vocab_size(), sp.seed)]
