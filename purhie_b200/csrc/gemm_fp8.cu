@@ -46,6 +46,7 @@ constexpr int THREADS = 192;                // copies, products, four epilogue w
 constexpr int A_BYTES = BM * BK;
 constexpr int FACTOR_BLOCKS = 32;           // blocks of K whose factors lie in shared memory at a time
 constexpr int MAX_SPLITS = 16;
+constexpr int MAX_ROWS = 1 << 30;           // of either operand: tiles are counted in 32 bits
 
 #define PH_ERR_FP8_PRODUCER 131
 #define PH_ERR_FP8_MMA 132
@@ -207,9 +208,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
                 tma_load_2d(smem_x + stage * BN * BK, &map_x, &full[stage], kb * BK, m0);
                 if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
-            // not past this point while copies may be in flight: the products have released every stage
-            for (int s = 0; s < STAGES && ok; ++s) {
-                if (!wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) break;
+            // not past this point while copies may be in flight: the products have released every stage, or, after a wait that ran
+            // out, the copies have at least arrived
+            for (int s = 0; s < STAGES; ++s) {
+                if (ok && !wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) ok = false;
+                if (!ok) wait(&full[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER);
                 if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
         }
@@ -481,8 +484,11 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
             }
-            for (int s = 0; s < STAGES && ok; ++s) {                  // not past this point while copies may be in flight
-                if (!wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) break;
+            // not past this point while copies may be in flight: the products have released every stage, or, after a wait that ran
+            // out, the copies of both CTAs have at least arrived (the leader sees them; the peer waits for it at the end)
+            for (int s = 0; s < STAGES; ++s) {
+                if (ok && !wait(&empty[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER)) ok = false;
+                if (!ok && leader) wait(&full[stage], phase ^ 1, flag, PH_ERR_FP8_PRODUCER);
                 if (++stage == STAGES) { stage = 0; phase ^= 1; }
             }
         } else if (threadIdx.x == 32 && leader) {
@@ -773,7 +779,7 @@ void choose(int M, int N, int K, int sms, bool whole, int* tile, int* splits) {
 // How ph_gemm_fp8 should cut an M x N x K product on the current device: *tile and *splits where they are 0 (the other one may be
 // given).  whole: the whole sum is wanted, not the parts.
 PH_EXPORT int ph_gemm_fp8_plan(int M, int N, int K, int whole, int* tile, int* splits) {
-    if (M < 1 || N < 1 || K < 1 || !tile || !splits || *tile < 0 || *splits < 0) return fail(PH_ERR_ARG, "gemm_fp8: no plan for M %d, N %d, K %d", M, N, K);
+    if (M < 1 || N < 1 || K < 1 || M > MAX_ROWS || N > MAX_ROWS || !tile || !splits || *tile < 0 || *splits < 0) return fail(PH_ERR_ARG, "gemm_fp8: no plan for M %d, N %d, K %d", M, N, K);
     const int kblocks = (K + BK - 1) / BK;
     if (*tile != 0 && *tile != 16 && *tile != 32 && *tile != 64 && *tile != 256) return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 256", *tile);
     if (*splits > kblocks || *splits > MAX_SPLITS) return fail(PH_ERR_ARG, "gemm_fp8: %d parts of K for %d blocks (at most %d)", *splits, kblocks, MAX_SPLITS);
@@ -791,6 +797,7 @@ PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const f
                           int splits, float* parts, int early_w, int* error_flag, cudaStream_t stream) {
     if (M == 0) return PH_OK;
     if (!x || !xs || !w || !ws || M < 1 || N < 1 || K < 1 || !valid_dtype(out_dtype)) return fail(PH_ERR_ARG, "gemm_fp8: bad arguments (M %d, N %d, K %d)", M, N, K);
+    if (M > MAX_ROWS || N > MAX_ROWS) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: operands of at most %d rows, not %d and %d", MAX_ROWS, M, N);
     if (K % 16) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: K = %d must be a multiple of 16 (16-byte rows for TMA)", K);
     if (((uintptr_t)x | (uintptr_t)w) & 15) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: operands must be 16-byte aligned");
     Params p = {};

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from purhie_b200.csrc import fp8
+from purhie_b200.csrc import fp8, ops
 from purhie_b200.native import KernelError
 
 E4M3 = torch.float8_e4m3fn
@@ -61,3 +61,53 @@ REFUSED = [
 def test_faces_refuse(text, call):
     with pytest.raises(KernelError, match=text):
         call()
+
+
+X, S = 1 << 20, 1 << 21          # addresses that nothing reads: every call below is refused on the host
+C_REFUSED = [
+    ("blocks are of", "ph_quantize_fp8", (X, 0, 8, X, S, 4, 8, 2, None)),
+    ("bad arguments", "ph_quantize_fp8", (X, 0, 7, X, S, 4, 8, 1, None)),
+    ("bad arguments", "ph_quantize_fp8", (X, 2, 8, X, S, 4, 8, 1, None)),
+    ("bad arguments", "ph_quantize_fp8", (None, 0, 8, X, S, 4, 8, 1, None)),
+    ("65535", "ph_quantize_fp8", (X, 0, 8, X, S, 65535 * 128 + 1, 8, 128, None)),
+    ("too many blocks", "ph_quantize_fp8", (X, 0, 4096, X, S, 2 ** 31 - 1, 4096, 1, None)),
+    ("at most 32768", "ph_add_rmsnorm_fp8", (X, None, 0, 1, 0, X, 1e-6, None, 1, 1, 32769, None, X, S, None)),
+    ("bad arguments", "ph_add_rmsnorm_fp8", (X, X, 0, 0, 64, X, 1e-6, None, 1, 1, 64, None, X, S, None)),
+    ("bad arguments", "ph_add_rmsnorm_fp8", (X, X, 0, 1, 64, X, float("nan"), None, 1, 1, 64, None, X, S, None)),
+    ("not kept", "ph_add_rmsnorm_fp8", (X, X, 0, 1, 64, X, 1e-6, X, 1, 1, 64, X, X, S, None)),
+    ("bad arguments", "ph_gated_fp8", (X, 0, 0, 0, X, S, 4, 8, None, None)),
+    ("gate 3", "ph_gated_fp8", (X, 0, 1, 0, X, S, 4, 8, (fp8.c_float * 4)(0, 0, 0, 3), None)),
+    ("too many blocks", "ph_gated_fp8", (X, 0, 1, 0, X, S, 2 ** 31 - 1, 256, None, None)),
+    ("multiple of 16", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 24, 16, 1, None, 0, None, None)),
+    ("aligned", "ph_gemm_fp8", (X + 8, S, X, S, X, 0, 4, 8, 32, 16, 1, None, 0, None, None)),
+    ("rows", "ph_gemm_fp8", (X, S, X, S, X, 0, 2 ** 31 - 1, 8, 32, 16, 1, None, 0, None, None)),
+    ("no room", "ph_gemm_fp8", (X, S, X, S, None, 0, 4, 8, 256, 16, 1, None, 0, None, None)),
+    ("no room", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 256, 16, 2, None, 0, None, None)),
+    ("summed here", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 256, 16, 2, X + 4, 0, None, None)),
+    ("parts of K", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 256, 16, 3, X, 0, None, None)),
+    ("tile 128", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 256, 128, 1, None, 0, None, None)),
+    ("no plan", "ph_gemm_fp8_plan", (0, 8, 32, 1, X, S)),
+    ("no plan", "ph_gemm_fp8_plan", (4, 8, 32, 1, None, S)),
+]
+
+
+@pytest.mark.parametrize("text,name,args", C_REFUSED, ids=[f"{i}-{n}" for i, (_, n, _) in enumerate(C_REFUSED)])
+def test_launchers_refuse(text, name, args):
+    with pytest.raises(KernelError, match=text):
+        ops.call("fp8", name, *args)
+
+
+@pytest.mark.parametrize("whole", [True, False])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 6144, 4096), (8, 4096, 12288), (64, 24576, 4096), (65, 100, 40000), (203, 1000, 2064),
+                                   (2048, 24576, 4096), (1 << 30, 8, 16), (4, 1 << 30, 16)])
+def test_plans(M, N, K, whole):
+    """What a plan gives can be launched, and what the caller gave stays."""
+    tile, splits = fp8.plan(M, N, K, whole=whole)
+    assert tile in (16, 32, 64, 256) and 1 <= splits <= min(16, -(-K // 128))
+    for given in (16, 256):
+        assert fp8.plan(M, N, K, tile=given)[0] == given
+    assert fp8.plan(M, N, K, splits=1)[1] == 1
+    with pytest.raises(KernelError, match="not one of"):
+        fp8.plan(M, N, K, tile=48)
+    with pytest.raises(KernelError, match="parts of K"):
+        fp8.plan(M, N, K, splits=17)
