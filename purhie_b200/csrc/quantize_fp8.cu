@@ -366,7 +366,8 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
 template <typename T> constexpr int MANY = 8 / (int)sizeof(T);
 
 // The number of blocks and of CTAs for them.  Several blocks a half warp once every SM has twice its fill of threads, else one: 2,048
-// rows of 12,288 gated bfloat16 values take 24.0 us with four, 29.9 with one and 34.7 with eight; 256 such rows 6.5 and 5.5.
+// rows of 12,288 gated bfloat16 values take 24.0 us with four, 29.9 with one and 34.7 with eight (and 26.7 where as many CTAs as the device holds walk over the blocks);
+// 256 such rows 6.5 and 5.5.
 inline bool count_blocks(long long rows, int width, int many, unsigned* blocks, int* u, unsigned* ctas) {
     const long long n = rows * ((width + BLOCK - 1) / BLOCK);
     if (n > 0x7fffffffLL - 4 * ROW_THREADS) return false;
