@@ -8,8 +8,9 @@
 // Everything in front of the rounding to 8 bits is float32.
 //
 // Half a warp owns a block of a row: 16 lanes of 8 values, read as 16-byte vectors (two for float32) and written as 8 bytes
-// a lane, the largest magnitude found by four exchanges.  Where rows do not lie on such boundaries (an odd width, a stride or
-// a base that is no multiple of 16 bytes) the lanes take every 16th value instead, one by one.  All three passes are bound by
+// a lane, the largest magnitude found by four exchanges.  Where rows do not lie on such boundaries (a width that is no multiple of
+// eight, a stride or a base that is no multiple of 16 bytes) a lane takes every 16th pair of values instead, or, where a pair does
+// not lie on its own boundary either (an odd width), every 16th value.  All three passes are bound by
 // memory: each input is read once and held in registers until its block's scale is known.
 // The reference's counterpart is its 8-bit activation blocks (src/matvec_q.hip), whose scales are per 32 values.
 #include "common.cuh"
@@ -50,8 +51,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
-// The place of a lane's value i inside its block.
-template <bool VEC> __device__ __forceinline__ int place(int lane16, int i) { return VEC ? lane16 * 8 + i : lane16 + 16 * i; }
+// The place of a lane's value i inside its block, for vectors of W values.
+template <int W> __device__ __forceinline__ int place(int lane16, int i) {
+    return W == 8 ? lane16 * 8 + i : W == 2 ? 32 * (i >> 1) + lane16 * 2 + (i & 1) : lane16 + 16 * i;
+}
 
 // A lane's eight values of a block as they lie in memory, and what is asked of them: a bfloat16 block waits for its scale in
 // half the registers, and its largest magnitude is found two values at a time.
@@ -63,6 +66,14 @@ template <> struct Held<float> {
         for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     }
     __device__ __forceinline__ void load(const float* p) { load8(p, v); }
+    __device__ __forceinline__ void load2(int i, const float* p) {                      // values 2 i and 2 i + 1
+        const float2 u = *reinterpret_cast<const float2*>(p);
+        v[2 * i] = u.x; v[2 * i + 1] = u.y;
+    }
+    __device__ __forceinline__ void load4(int i, const float* p) {                      // values 4 i .. 4 i + 3
+        const float4 u = *reinterpret_cast<const float4*>(p);
+        v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
+    }
     __device__ __forceinline__ void set(int i, float x) { v[i] = x; }
     __device__ __forceinline__ float get(int i) const { return v[i]; }
     __device__ __forceinline__ float largest() const {
@@ -79,6 +90,11 @@ template <> struct Held<__nv_bfloat16> {
         const uint4 u = *reinterpret_cast<const uint4*>(p);
         v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
     }
+    __device__ __forceinline__ void load2(int i, const __nv_bfloat16* p) { v[i] = *reinterpret_cast<const uint32_t*>(p); }
+    __device__ __forceinline__ void load4(int i, const __nv_bfloat16* p) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        v[2 * i] = u.x; v[2 * i + 1] = u.y;
+    }
     __device__ __forceinline__ void set(int i, __nv_bfloat16 x) {
         const uint32_t bits = __bfloat16_as_ushort(x);
         v[i >> 1] = (i & 1) ? (v[i >> 1] & 0xffffu) | bits << 16 : (v[i >> 1] & 0xffff0000u) | bits;
@@ -93,56 +109,68 @@ template <> struct Held<__nv_bfloat16> {
 };
 
 // A lane's eight values of the block that starts at column k0 of a row of K (zeros behind the row's end).
-template <bool VEC, typename T>
+template <int W, typename T>
 __device__ __forceinline__ void hold_block(const T* row, int k0, int lane16, int K, Held<T>& h) {
     h.clear();
-    if (VEC) {
+    if (W == 8) {
         if (k0 + lane16 * 8 < K) h.load(row + k0 + lane16 * 8);
+    } else if (W == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = k0 + place<2>(lane16, 2 * i);
+            if (k < K) h.load2(i, row + k);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int k = k0 + place<false>(lane16, i);
+            const int k = k0 + place<1>(lane16, i);
             if (k < K) h.set(i, row[k]);
         }
     }
 }
-template <bool VEC, typename T>
+template <int W, typename T>
 __device__ __forceinline__ void load_block(const T* row, int k0, int lane16, int K, float* v) {
     Held<T> h;
-    hold_block<VEC>(row, k0, lane16, K, h);
+    hold_block<W>(row, k0, lane16, K, h);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = h.get(i);
 }
 
-template <bool VEC, typename V>
+template <int W, typename V>
 __device__ __forceinline__ void store_block(uint8_t* row, int k0, int lane16, int K, const V& v, float inverse) {
     uint32_t p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[i] = pack2(v.get(2 * i) * inverse, v.get(2 * i + 1) * inverse);
-    if (VEC) {
+    if (W == 8) {
         if (k0 + lane16 * 8 < K) *(uint2*)(row + k0 + lane16 * 8) = make_uint2(p[0] | p[1] << 16, p[2] | p[3] << 16);
+    } else if (W == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = k0 + place<2>(lane16, 2 * i);
+            if (k < K) *(uint16_t*)(row + k) = (uint16_t)p[i];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int k = k0 + place<false>(lane16, i);
+            const int k = k0 + place<1>(lane16, i);
             if (k < K) row[k] = (uint8_t)(p[i >> 1] >> (8 * (i & 1)));
         }
     }
 }
 
 // A lane's share of a block: the block's scale to *scale, its values to the row.  Every lane of the warp calls this.
-template <bool VEC, typename V>
+template <int W, typename V>
 __device__ __forceinline__ void finish_block(uint8_t* row, float* scale, bool live, int k0, int lane16, int K, const V& v) {
     const float a = max_nan(half_warp_max(v.largest()), LEAST);
     if (!live) return;
     if (lane16 == 0) *scale = a / TOP;
-    store_block<VEC>(row, k0, lane16, K, v, TOP / a);
+    store_block<W>(row, k0, lane16, K, v, TOP / a);
 }
 
 constexpr int ROW_THREADS = 256;
 
 // U neighbouring blocks of rows for each half warp, all of them asked for before the first is worked on.
-template <typename T, bool VEC, int U>
+template <typename T, int W, int U>
 __global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __restrict__ x, long long stride, uint8_t* __restrict__ q, float* __restrict__ scales, unsigned blocks,
                                      unsigned kblocks, int K) {
     pdl_launch_dependents();
@@ -157,17 +185,17 @@ __global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const T* __r
     for (int u = 0; u < U; ++u) {
         at_row[u] = row;
         k0[u] = (int)b * BLOCK;
-        if (first + u < blocks) hold_block<VEC>(x + row * stride, k0[u], lane16, K, v[u]);
+        if (first + u < blocks) hold_block<W>(x + row * stride, k0[u], lane16, K, v[u]);
         else v[u].clear();
         if (++b == kblocks) { b = 0; ++row; }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        finish_block<VEC>(q + (size_t)at_row[u] * K, scales + first + u, first + u < blocks, k0[u], lane16, K, v[u]);
+        finish_block<W>(q + (size_t)at_row[u] * K, scales + first + u, first + u < blocks, k0[u], lane16, K, v[u]);
 }
 
 // One CTA for each 128 x 128 block of a weight: 16 half warps, eight rows each.
-template <typename T, bool VEC>
+template <typename T, int W>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, long long stride, uint8_t* __restrict__ q, float* __restrict__ scales, int T_rows, int K) {
     __shared__ float part[8];
     pdl_wait();
@@ -178,7 +206,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
         const long long t = t0 + r * 16 + half;
-        if (t < T_rows) hold_block<VEC>(x + t * stride, k0, lane16, K, v[r]);
+        if (t < T_rows) hold_block<W>(x + t * stride, k0, lane16, K, v[r]);
         else v[r].clear();
     }
     float m = v[0].largest();
@@ -196,7 +224,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
         const long long t = t0 + r * 16 + half;
-        if (t < T_rows) store_block<VEC>(q + t * K, k0, lane16, K, v[r], inverse);
+        if (t < T_rows) store_block<W>(q + t * K, k0, lane16, K, v[r], inverse);
     }
 }
 
@@ -216,7 +244,7 @@ struct NormParams {
     float* scales;
 };
 
-template <typename A, bool VEC, int U>
+template <typename A, int W, int U>
 __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(NormParams p) {
     __shared__ float scratch[32];
     const int lane16 = threadIdx.x & 15, half = threadIdx.x >> 4, halves = blockDim.x >> 4;
@@ -229,13 +257,13 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(NormParams p) {
     const A* add = (const A*)p.add + t * p.E;
     float v[U][8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_block<VEC>(x, (half + u * halves) * BLOCK, lane16, p.E, v[u]);
+    for (int u = 0; u < U; ++u) load_block<W>(x, (half + u * halves) * BLOCK, lane16, p.E, v[u]);
     if (p.add) {
         for (int s = 0; s < p.parts; ++s) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float a[8];
-                load_block<VEC>(add + s * p.part_stride, (half + u * halves) * BLOCK, lane16, p.E, a);
+                load_block<W>(add + s * p.part_stride, (half + u * halves) * BLOCK, lane16, p.E, a);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[u][i] += a[i];
             }
@@ -251,12 +279,16 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(NormParams p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k0 = (half + u * halves) * BLOCK;
-            if (VEC) {
+            if (W == 8) {
                 if (k0 + lane16 * 8 < p.E) store8(o + k0 + lane16 * 8, v[u]);
+            } else if (W == 2) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2)
+                    if (k0 + place<2>(lane16, i) < p.E) *(float2*)(o + k0 + place<2>(lane16, i)) = make_float2(v[u][i], v[u][i + 1]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (k0 + place<false>(lane16, i) < p.E) o[k0 + place<false>(lane16, i)] = v[u][i];
+                    if (k0 + place<1>(lane16, i) < p.E) o[k0 + place<1>(lane16, i)] = v[u][i];
             }
         }
     }
@@ -265,11 +297,11 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(NormParams p) {
     for (int u = 0; u < U; ++u) {
         const int b = half + u * halves;
         float w[8];
-        load_block<VEC>(p.weight, b * BLOCK, lane16, p.E, w);
+        load_block<W>(p.weight, b * BLOCK, lane16, p.E, w);
         Held<float> y;
 #pragma unroll
         for (int i = 0; i < 8; ++i) y.v[i] = v[u][i] * f * w[i];
-        finish_block<VEC>(p.q + r * p.E, p.scales + r * p.kblocks + b, b < p.kblocks, b * BLOCK, lane16, p.E, y);
+        finish_block<W>(p.q + r * p.E, p.scales + r * p.kblocks + b, b < p.kblocks, b * BLOCK, lane16, p.E, y);
     }
 }
 
@@ -289,7 +321,7 @@ __device__ __forceinline__ float gated_value(const Gate& gate, float g, float u)
 }
 
 // Rows of (g0, u0, g1, u1, ...), in `parts` parts that are summed first, to gated rows of F in 8 bits; U blocks for each half warp.
-template <typename T, bool VEC, int U>
+template <typename T, int W, int U>
 __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restrict__ gate_up, int parts, long long part_stride, uint8_t* __restrict__ q, float* __restrict__ scales,
                                  unsigned blocks, unsigned kblocks, int F, Gate gate) {
     pdl_launch_dependents();
@@ -297,7 +329,8 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
     const int lane16 = threadIdx.x & 15;
     const unsigned first = (blockIdx.x * (ROW_THREADS / 16) + (threadIdx.x >> 4)) * U;
     unsigned row = first / kblocks, b = first - row * kblocks;
-    if (VEC && parts == 1) {
+    const bool pairs = ((uintptr_t)gate_up & (2 * sizeof(T) - 1)) == 0;       // (a pair never straddles its own boundary then)
+    if (parts == 1) {
         // one part: what is read waits as it lies in memory
         Held<T> v[U][2];
         unsigned at_row[U];
@@ -308,10 +341,30 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
             k0[u] = (int)b * BLOCK;
             v[u][0].clear();
             v[u][1].clear();
-            if (first + u < blocks && k0[u] + lane16 * 8 < F) {
-                const T* src = gate_up + (size_t)row * 2 * F + 2 * (k0[u] + lane16 * 8);
-                v[u][0].load(src);
-                v[u][1].load(src + 8);
+            const T* src = gate_up + (size_t)row * 2 * F;
+            if (first + u >= blocks) {
+            } else if (W == 8) {
+                if (k0[u] + lane16 * 8 < F) {
+                    v[u][0].load(src + 2 * (k0[u] + lane16 * 8));
+                    v[u][1].load(src + 2 * (k0[u] + lane16 * 8) + 8);
+                }
+            } else if (W == 2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = k0[u] + place<2>(lane16, 2 * i);
+                    if (k < F) v[u][i >> 1].load4(i & 1, src + 2 * (size_t)k);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = k0[u] + place<1>(lane16, i);
+                    if (k >= F) continue;
+                    if (pairs) v[u][i >> 2].load2(i & 3, src + 2 * (size_t)k);
+                    else {
+                        v[u][i >> 2].set(2 * (i & 3), src[2 * (size_t)k]);
+                        v[u][i >> 2].set(2 * (i & 3) + 1, src[2 * (size_t)k + 1]);
+                    }
+                }
             }
             if (++b == kblocks) { b = 0; ++row; }
         }
@@ -320,7 +373,7 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
             Held<float> h;
 #pragma unroll
             for (int i = 0; i < 8; ++i) h.v[i] = gated_value(gate, v[u][i >> 2].get(2 * (i & 3)), v[u][i >> 2].get(2 * (i & 3) + 1));
-            finish_block<VEC>(q + (size_t)at_row[u] * F, scales + first + u, first + u < blocks, k0[u], lane16, F, h);
+            finish_block<W>(q + (size_t)at_row[u] * F, scales + first + u, first + u < blocks, k0[u], lane16, F, h);
         }
         return;
     }
@@ -330,7 +383,7 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
         const bool live = first + u < blocks;
         const T* src = gate_up + (size_t)row * 2 * F;
         Held<float> h;
-        if (VEC) {
+        if (W == 8) {
             float g[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) g[i] = 0.0f;
@@ -348,7 +401,7 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int k = k0 + place<false>(lane16, i);
+                const int k = k0 + place<W>(lane16, i);
                 float g = 0.0f, x = 0.0f;
                 if (live && k < F) {
                     g = to_float<T>(src[2 * (size_t)k]); x = to_float<T>(src[2 * (size_t)k + 1]);
@@ -357,7 +410,7 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
                 h.v[i] = gated_value(gate, g, x);
             }
         }
-        finish_block<VEC>(q + (size_t)row * F, scales + first + u, live, k0, lane16, F, h);
+        finish_block<W>(q + (size_t)row * F, scales + first + u, live, k0, lane16, F, h);
         if (++b == kblocks) { b = 0; ++row; }
     }
 }
@@ -379,7 +432,7 @@ inline bool count_blocks(long long rows, int width, int many, unsigned* blocks, 
 
 inline bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
-template <typename A, bool VEC>
+template <typename A, int W>
 int launch_norm(const NormParams& p, int n, cudaStream_t stream) {
     // blocks per half warp: as few as a CTA of 1,024 threads allows, so that a row is spread wide and waits for its sum the
     // shortest (2,048 rows of 5,120: 20.5 us with one, 24.5 with two, 29.8 with four)
@@ -387,9 +440,9 @@ int launch_norm(const NormParams& p, int n, cudaStream_t stream) {
     const int halves = (p.kblocks + u - 1) / u;
     const int threads = (halves * 16 + 31) / 32 * 32;
     switch (u) {
-        case 1: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 1>, dim3(n), dim3(threads), 0, stream, p); break;
-        case 2: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 2>, dim3(n), dim3(threads), 0, stream, p); break;
-        default: launch_overlapped(add_rmsnorm_fp8_kernel<A, VEC, 4>, dim3(n), dim3(threads), 0, stream, p); break;
+        case 1: launch_overlapped(add_rmsnorm_fp8_kernel<A, W, 1>, dim3(n), dim3(threads), 0, stream, p); break;
+        case 2: launch_overlapped(add_rmsnorm_fp8_kernel<A, W, 2>, dim3(n), dim3(threads), 0, stream, p); break;
+        default: launch_overlapped(add_rmsnorm_fp8_kernel<A, W, 4>, dim3(n), dim3(threads), 0, stream, p); break;
     }
     return check_launch("add_rmsnorm_fp8");
 }
@@ -403,13 +456,13 @@ PH_EXPORT int ph_quantize_fp8(const void* x, int dtype, long long stride, void* 
     if (block_rows != 1 && block_rows != BLOCK) return fail(PH_ERR_ARG, "quantize_fp8: blocks are of 1 or 128 rows, not %d", block_rows);
     const int kblocks = (K + BLOCK - 1) / BLOCK;
     const int size = dtype == PH_F32 ? 4 : 2;
-    const bool vec = K % 8 == 0 && (stride * size) % 16 == 0 && aligned(x, 16) && aligned(q, 8);
+    const int w = K % 8 == 0 && (stride * size) % 16 == 0 && aligned(x, 16) && aligned(q, 8) ? 8 : K % 2 == 0 && stride % 2 == 0 && aligned(x, 2 * size) && aligned(q, 2) ? 2 : 1;
     if (block_rows == BLOCK) {
         if ((T + BLOCK - 1) / BLOCK > 65535) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: a weight of at most 65535 * 128 rows, not %d", T);
         const dim3 grid(kblocks, (T + BLOCK - 1) / BLOCK);
         PH_DISPATCH(dtype, X, {
-            if (vec) launch_overlapped(quantize_blocks_kernel<X, true>, grid, dim3(256), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, T, K);
-            else launch_overlapped(quantize_blocks_kernel<X, false>, grid, dim3(256), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, T, K);
+            auto kernel = w == 8 ? quantize_blocks_kernel<X, 8> : w == 2 ? quantize_blocks_kernel<X, 2> : quantize_blocks_kernel<X, 1>;
+            launch_overlapped(kernel, grid, dim3(256), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, T, K);
         });
         return check_launch("quantize_fp8");
     }
@@ -418,8 +471,9 @@ PH_EXPORT int ph_quantize_fp8(const void* x, int dtype, long long stride, void* 
     int u;
     if (!count_blocks(T, K, many, &blocks, &u, &ctas)) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: %d x %d are too many blocks", T, K);
     PH_DISPATCH(dtype, X, {
-        auto kernel = vec ? (u == 1 ? quantize_rows_kernel<X, true, 1> : quantize_rows_kernel<X, true, MANY<X>>)
-                          : (u == 1 ? quantize_rows_kernel<X, false, 1> : quantize_rows_kernel<X, false, MANY<X>>);
+        auto kernel = w == 8 ? (u == 1 ? quantize_rows_kernel<X, 8, 1> : quantize_rows_kernel<X, 8, MANY<X>>)
+                    : w == 2 ? (u == 1 ? quantize_rows_kernel<X, 2, 1> : quantize_rows_kernel<X, 2, MANY<X>>)
+                             : (u == 1 ? quantize_rows_kernel<X, 1, 1> : quantize_rows_kernel<X, 1, MANY<X>>);
         launch_overlapped(kernel, dim3(ctas), dim3(ROW_THREADS), 0, stream, (const X*)x, stride, (uint8_t*)q, scales, blocks, (unsigned)kblocks, K);
     });
     return check_launch("quantize_fp8");
@@ -437,8 +491,9 @@ PH_EXPORT int ph_add_rmsnorm_fp8(const float* x, const void* add, int add_dtype,
     if (kblocks > 256) return fail(PH_ERR_UNSUPPORTED, "add_rmsnorm_fp8: rows of at most 32768 values, not %d", E);
     NormParams p = {x, add, parts, part_stride, weight, eps, rows, T, E, kblocks, x_out, (uint8_t*)q, scales};
     const int size = add_dtype == PH_F32 ? 4 : 2;
-    const bool vec = E % 8 == 0 && aligned(x, 16) && aligned(weight, 16) && aligned(x_out, 16) && aligned(q, 8) && aligned(add, 16) && (part_stride * size) % 16 == 0;
-    PH_DISPATCH(add_dtype, A, { return vec ? launch_norm<A, true>(p, n, stream) : launch_norm<A, false>(p, n, stream); });
+    const bool v8 = E % 8 == 0 && aligned(x, 16) && aligned(weight, 16) && aligned(x_out, 16) && aligned(q, 8) && aligned(add, 16) && (part_stride * size) % 16 == 0;
+    const bool v2 = E % 2 == 0 && aligned(x, 8) && aligned(weight, 8) && aligned(x_out, 8) && aligned(q, 2) && aligned(add, 2 * size) && part_stride % 2 == 0;
+    PH_DISPATCH(add_dtype, A, { return v8 ? launch_norm<A, 8>(p, n, stream) : v2 ? launch_norm<A, 2>(p, n, stream) : launch_norm<A, 1>(p, n, stream); });
 }
 
 // gate_up [parts][T, 2 F] (part_stride elements apart) of (gate, up) pairs to q [T, F] and scales [T, ceil(F / 128)].  gate: null
@@ -455,10 +510,11 @@ PH_EXPORT int ph_gated_fp8(const void* gate_up, int dtype, int parts, long long 
     unsigned blocks, ctas;
     int u;
     if (!count_blocks(T, F, many, &blocks, &u, &ctas)) return fail(PH_ERR_UNSUPPORTED, "gated_fp8: %d x %d are too many blocks", T, F);
-    const bool vec = F % 8 == 0 && aligned(gate_up, 16) && aligned(q, 8) && (part_stride * size) % 16 == 0;
+    const int w = F % 8 == 0 && aligned(gate_up, 16) && aligned(q, 8) && (part_stride * size) % 16 == 0 ? 8 : F % 2 == 0 && aligned(gate_up, 4 * size) && aligned(q, 2) ? 2 : 1;
     PH_DISPATCH(dtype, X, {
-        auto kernel = vec ? (u == 1 ? gated_fp8_kernel<X, true, 1> : gated_fp8_kernel<X, true, MANY<X>>)
-                          : (u == 1 ? gated_fp8_kernel<X, false, 1> : gated_fp8_kernel<X, false, MANY<X>>);
+        auto kernel = w == 8 ? (u == 1 ? gated_fp8_kernel<X, 8, 1> : gated_fp8_kernel<X, 8, MANY<X>>)
+                    : w == 2 ? (u == 1 ? gated_fp8_kernel<X, 2, 1> : gated_fp8_kernel<X, 2, MANY<X>>)
+                             : (u == 1 ? gated_fp8_kernel<X, 1, 1> : gated_fp8_kernel<X, 1, MANY<X>>);
         launch_overlapped(kernel, dim3(ctas), dim3(ROW_THREADS), 0, stream, (const X*)gate_up, parts, part_stride, (uint8_t*)q, scales, blocks, (unsigned)kblocks, F, g);
     });
     return check_launch("gated_fp8");

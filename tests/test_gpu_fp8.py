@@ -55,7 +55,7 @@ def plain_quantize(x, rows):
     return (x.float() * spread(top / a, rows, *x.shape)).to(torch.float8_e4m3fn), a / top
 
 
-SIZES = [(1, 1), (1, 128), (3, 127), (2, 129), (5, 264), (128, 256), (129, 1000), (300, 4096), (257, 131)]
+SIZES = [(1, 1), (1, 128), (3, 127), (2, 129), (5, 264), (128, 256), (129, 1000), (300, 4096), (257, 131), (131, 1002), (6, 262)]
 
 
 @pytest.mark.parametrize("rows", [1, 128])
@@ -72,7 +72,7 @@ def test_quantize(T, K, dtype, rows):
 
 
 @pytest.mark.parametrize("rows", [1, 128])
-@pytest.mark.parametrize("off,stride", [(0, 1040), (8, 1040), (1, 1040), (8, 1003)])
+@pytest.mark.parametrize("off,stride", [(0, 1040), (8, 1040), (2, 1040), (2, 1002), (1, 1040), (8, 1003)])
 def test_quantize_of_strided_rows(off, stride, rows):
     from purhie_b200.csrc import fp8
     held = rnd(200, stride, seed=1).to(torch.bfloat16)
@@ -120,7 +120,7 @@ def test_rows_past_two_to_the_31():
     assert torch.equal(q.view(torch.uint8), wq.view(torch.uint8)) and torch.equal(s, ws)
 
 
-@pytest.mark.parametrize("E", [1, 64, 127, 128, 1000, 2056, 4096, 5120, 8200, 16400, 32768])
+@pytest.mark.parametrize("E", [1, 64, 127, 128, 1000, 1002, 2056, 4096, 5120, 8200, 16400, 32768])
 @pytest.mark.parametrize("add,parts", [(None, 1), ("f32", 1), ("bf16", 1), ("f32", 3)])
 def test_add_rmsnorm(E, add, parts):
     from purhie_b200.csrc import fp8
@@ -178,7 +178,7 @@ def gate_value(g, u, gate):
 
 @pytest.mark.parametrize("gate", [None, (1.702, 7.0, 1.0), "gelu_tanh"])
 @pytest.mark.parametrize("dtype,parts", [("f32", 1), ("bf16", 1), ("f32", 3)])
-@pytest.mark.parametrize("T,F", [(1, 1), (3, 127), (2, 128), (5, 1000), (4, 1001), (33, 4104)])
+@pytest.mark.parametrize("T,F", [(1, 1), (3, 127), (2, 128), (5, 1000), (4, 1001), (7, 1002), (33, 4104)])
 def test_gated(T, F, dtype, parts, gate):
     from purhie_b200.csrc import fp8
     gu = rnd(parts, T, 2 * F, seed=T + F, scale=4.0).to(DT[dtype])
@@ -193,6 +193,26 @@ def test_gated(T, F, dtype, parts, gate):
     tiny = (num * up).abs() * 2.0 ** -125
     rel = rel + tiny / h.abs().clamp(min=1e-300)
     check_quantized(q, s, h, 1, rel)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("F", [1000, 1002, 1001])
+@pytest.mark.parametrize("T", [3, 5200])
+def test_inputs_off_their_boundaries(T, F, dtype):
+    """Rows that start one, two and four values behind a boundary, few and many of them, give what aligned ones give."""
+    from purhie_b200.csrc import fp8
+    gu, x, ones = rnd(T, 2 * F, seed=F, scale=3.0).to(DT[dtype]), rnd(T, F, seed=F + 1).to(DT[dtype]), torch.ones(F, device=DEV)
+    want_g, want_x, want_n = fp8.gated(gu), fp8.quantize(x), fp8.add_rmsnorm(x.float(), x, ones, 1e-6, write_x=False)
+    for off in (1, 2, 4):
+        def moved(t):
+            y = torch.empty(t.numel() + 8, dtype=t.dtype, device=DEV)[off:off + t.numel()].view(t.shape)
+            return y.copy_(t)
+        for got, want in ((fp8.gated(moved(gu)), want_g), (fp8.quantize(moved(x)), want_x)):
+            assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(got[1], want[1])
+        # a row's sum of squares is added up in another order: its factor is some roundings off, and a value may fall to its neighbour
+        q, s = fp8.add_rmsnorm(moved(x.float()), moved(x), ones, 1e-6, write_x=False)
+        assert ((s - want_n[1]).abs() <= 100 * U * s).all()
+        assert ((q.float() - want_n[0].float()).abs() <= want_n[0].float().abs().clamp(min=2.0 ** -6) * 2.0 ** -3).all()
 
 
 def test_gated_keeps_what_is_not_a_number():
