@@ -46,7 +46,7 @@ constexpr int THREADS = 192;                // copies, products, four epilogue w
 constexpr int A_BYTES = BM * BK;
 constexpr int FACTOR_BLOCKS = 32;           // blocks of K whose factors lie in shared memory at a time
 constexpr int MAX_SPLITS = 16;
-constexpr int MAX_ROWS = 1 << 30;           // of either operand: tiles are counted in 32 bits
+constexpr int MAX_SIZE = 1 << 30;           // of M, N and K: tiles and blocks are counted in 32 bits
 
 #define PH_ERR_FP8_PRODUCER 131
 #define PH_ERR_FP8_MMA 132
@@ -365,7 +365,7 @@ constexpr int PAIR_STAGES = 4;
 constexpr int PAIR_WARPS = 8;
 constexpr int PAIR_THREADS = 128 + 32 * PAIR_WARPS;
 // Registers a thread: the launch gives each of the 384 threads 168 (what 65,536 hold), the four warps of copies and products hand
-// most of theirs back and the epilogue's take them: 128 * 40 + 256 * 232 = 384 * 168.
+// most of theirs back and the epilogue's take them: 128 * 56 + 256 * 224 = 384 * 168.
 constexpr int PAIR_REGS = 168, PAIR_REGS_LOW = 56, PAIR_REGS_HIGH = 224;
 static_assert(128 * PAIR_REGS_LOW + 32 * PAIR_WARPS * PAIR_REGS_HIGH <= PAIR_THREADS * PAIR_REGS, "more registers than the launch has");
 constexpr int PAIR_BOX_BYTES = 32 * 128;                          // 32 rows of 128 bytes on their way out
@@ -788,7 +788,7 @@ void choose(int M, int N, int K, int sms, bool whole, int* tile, int* splits) {
 // How ph_gemm_fp8 should cut an M x N x K product on the current device: *tile and *splits where they are 0 (the other one may be
 // given).  whole: the whole sum is wanted, not the parts.
 PH_EXPORT int ph_gemm_fp8_plan(int M, int N, int K, int whole, int* tile, int* splits) {
-    if (M < 1 || N < 1 || K < 1 || M > MAX_ROWS || N > MAX_ROWS || !tile || !splits || *tile < 0 || *splits < 0) return fail(PH_ERR_ARG, "gemm_fp8: no plan for M %d, N %d, K %d", M, N, K);
+    if (M < 1 || N < 1 || K < 1 || M > MAX_SIZE || N > MAX_SIZE || K > MAX_SIZE || !tile || !splits || *tile < 0 || *splits < 0) return fail(PH_ERR_ARG, "gemm_fp8: no plan for M %d, N %d, K %d", M, N, K);
     const int kblocks = (K + BK - 1) / BK;
     if (*tile != 0 && *tile != 16 && *tile != 32 && *tile != 64 && *tile != 256) return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 256", *tile);
     if (*splits > kblocks || *splits > MAX_SPLITS) return fail(PH_ERR_ARG, "gemm_fp8: %d parts of K for %d blocks (at most %d)", *splits, kblocks, MAX_SPLITS);
@@ -806,7 +806,7 @@ PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const f
                           int splits, float* parts, int early_w, int* error_flag, cudaStream_t stream) {
     if (M == 0) return PH_OK;
     if (!x || !xs || !w || !ws || M < 1 || N < 1 || K < 1 || !valid_dtype(out_dtype)) return fail(PH_ERR_ARG, "gemm_fp8: bad arguments (M %d, N %d, K %d)", M, N, K);
-    if (M > MAX_ROWS || N > MAX_ROWS) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: operands of at most %d rows, not %d and %d", MAX_ROWS, M, N);
+    if (M > MAX_SIZE || N > MAX_SIZE || K > MAX_SIZE) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: M, N and K of at most %d, not %d, %d and %d", MAX_SIZE, M, N, K);
     if (K % 16) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: K = %d must be a multiple of 16 (16-byte rows for TMA)", K);
     if (((uintptr_t)x | (uintptr_t)w) & 15) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8: operands must be 16-byte aligned");
     Params p = {};

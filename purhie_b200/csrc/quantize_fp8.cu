@@ -23,6 +23,7 @@ namespace {
 using namespace ph;
 
 constexpr int BLOCK = 128;
+constexpr int MAX_WIDTH = 1 << 30;                             // of a row: its blocks are counted in 32 bits
 constexpr float TOP = 448.0f;                                  // the largest e4m3 value
 constexpr float LEAST = 448.0f * 1.17549435e-38f;              // 448 * 2^-126
 
@@ -453,12 +454,13 @@ int launch_norm(const NormParams& p, int n, cudaStream_t stream) {
 PH_EXPORT int ph_quantize_fp8(const void* x, int dtype, long long stride, void* q, float* scales, int T, int K, int block_rows, cudaStream_t stream) {
     if (T == 0) return PH_OK;
     if (!x || !q || !scales || T < 0 || K < 1 || stride < K || !valid_dtype(dtype)) return fail(PH_ERR_ARG, "quantize_fp8: bad arguments (T %d, K %d, row stride %lld)", T, K, stride);
+    if (K > MAX_WIDTH) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: rows of at most %d values, not %d", MAX_WIDTH, K);
     if (block_rows != 1 && block_rows != BLOCK) return fail(PH_ERR_ARG, "quantize_fp8: blocks are of 1 or 128 rows, not %d", block_rows);
     const int kblocks = (K + BLOCK - 1) / BLOCK;
     const int size = dtype == PH_F32 ? 4 : 2;
     const int w = K % 8 == 0 && (stride * size) % 16 == 0 && aligned(x, 16) && aligned(q, 8) ? 8 : K % 2 == 0 && stride % 2 == 0 && aligned(x, 2 * size) && aligned(q, 2) ? 2 : 1;
     if (block_rows == BLOCK) {
-        if ((T + BLOCK - 1) / BLOCK > 65535) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: a weight of at most 65535 * 128 rows, not %d", T);
+        if (T > 65535 * BLOCK) return fail(PH_ERR_UNSUPPORTED, "quantize_fp8: a weight of at most 65535 * 128 rows, not %d", T);
         const dim3 grid(kblocks, (T + BLOCK - 1) / BLOCK);
         PH_DISPATCH(dtype, X, {
             auto kernel = w == 8 ? quantize_blocks_kernel<X, 8> : w == 2 ? quantize_blocks_kernel<X, 2> : quantize_blocks_kernel<X, 1>;

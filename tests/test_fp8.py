@@ -80,7 +80,10 @@ C_REFUSED = [
     ("too many blocks", "ph_gated_fp8", (X, 0, 1, 0, X, S, 2 ** 31 - 1, 256, None, None)),
     ("multiple of 16", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 24, 16, 1, None, 0, None, None)),
     ("aligned", "ph_gemm_fp8", (X + 8, S, X, S, X, 0, 4, 8, 32, 16, 1, None, 0, None, None)),
-    ("rows", "ph_gemm_fp8", (X, S, X, S, X, 0, 2 ** 31 - 1, 8, 32, 16, 1, None, 0, None, None)),
+    ("at most", "ph_quantize_fp8", (X, 0, 2 ** 31 - 1, X, S, 1, 2 ** 31 - 1, 1, None)),
+    ("65535", "ph_quantize_fp8", (X, 0, 8, X, S, 2 ** 31 - 1, 8, 128, None)),
+    ("at most", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 2 ** 31 - 16, 16, 1, None, 0, None, None)),
+    ("at most", "ph_gemm_fp8", (X, S, X, S, X, 0, 2 ** 31 - 1, 8, 32, 16, 1, None, 0, None, None)),
     ("no room", "ph_gemm_fp8", (X, S, X, S, None, 0, 4, 8, 256, 16, 1, None, 0, None, None)),
     ("no room", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 256, 16, 2, None, 0, None, None)),
     ("summed here", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 256, 16, 2, X + 4, 0, None, None)),

@@ -196,3 +196,29 @@ def test_matrices_that_do_not_fit_stay_as_they_are(tmp_path):
     narrow, _ = feed_forward_probe(tmp_path, 264, 648, None, {"gemm": "fp8"})
     same, _ = feed_forward_probe(tmp_path, 264, 648, None, {"gemm": "auto"})
     assert np.array_equal(narrow.feed_forward(x), same.feed_forward(x))
+
+
+@pytest.mark.parametrize("design", ["bozosun", "sizizen", "zerusun", "vokepel", "noditar", "defapel"])
+@pytest.mark.parametrize("which", ["CONFIG_A", "CONFIG_C"])
+def test_every_design_loads_and_answers(design, which):
+    """What the other designs' parts do with the option: attention and feed-forwards in 8 bits, the rest as it is.  Logits are near
+    those in bfloat16 (a scale or a layout that is wrong would move them by their own size; a token that takes another expert moves
+    its own row, so the middle row is looked at)."""
+    import importlib
+    from purhie_b200.api import load_model_random
+    config = getattr(importlib.import_module(f"{design}_helpers"), which)
+    tokens = random_tokens(80, config["vocab"], 3)
+    got = {}
+    for gemm in ("auto", "fp8"):
+        model = load_model_random(config, 5, "bfloat16", std=0.1, options={"gemm": gemm})
+        model.kv_cache_init(96, max_sequences=2)
+        rows = [model.prefill_logits(tokens[:50]), model.prefill_logits(tokens[50:70])]
+        for t in tokens[70:]:
+            model.decode_token(t)
+            rows.append(model.get_logits()[None])
+        model.synchronize()
+        model.free()
+        got[gemm] = np.concatenate(rows).astype(np.float64)
+    assert np.isfinite(got["fp8"]).all()
+    far = np.linalg.norm(got["fp8"] - got["auto"], axis=1) / np.linalg.norm(got["auto"], axis=1)
+    assert np.median(far) < 0.3, far
