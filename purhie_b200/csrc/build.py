@@ -1,7 +1,8 @@
 """Compiling the CUDA sources for sm_100a and loading the libraries.
 
 Each *library* is a handful of ``.cu`` files compiled by ``nvcc`` into one shared object next to the
-sources (``_build/``), without any Python or torch header, and loaded with ``ctypes``.  A library is
+sources (``_build/``), without any Python or torch header, and loaded with ``ctypes`` (``fp8_calls`` alone
+is an extension module that knows torch).  A library is
 compiled the first time something needs it, so a float32 run compiles the plain kernels only; while it
 compiles, a line is printed now and then.  If the package folder cannot be written, a per-user folder
 under the temporary directory is used.  A missing compiler or a failed compile raises: there is no
@@ -65,6 +66,13 @@ LIBRARIES: Dict[str, dict] = {
         "flags": [],
         "link": [],
     },
+    # the plain calls of fp8.py's faces, checks to launch in one step: an extension module, the one library that knows torch
+    "fp8_calls": {
+        "sources": ["fp8_calls.cpp"],
+        "flags": lambda: _torch_flags()[0],
+        "link": lambda: _torch_flags()[1],
+        "file_name": "fp8_calls.so",
+    },
     # the host library: configuration, weights, parts, cache manager, step function, scheduler, samplers and the C
     # API (api/inference.h); it opens the kernel libraries above by need, from the folder it is loaded from
     "qengine": {
@@ -94,8 +102,25 @@ LIBRARIES: Dict[str, dict] = {
     },
 }
 
+def _torch_flags():
+    """How an extension module that uses torch is compiled and linked."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    include, lib = os.path.join(root, "include"), os.path.join(root, "lib")
+    return (["-I", include, "-I", os.path.join(include, "torch", "csrc", "api", "include"), "-I", sysconfig.get_paths()["include"],
+             f"-DPH_TORCH_VERSION={torch.__version__}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"],
+            ["-L", lib, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"])
+
+
+def _flags(spec: dict, which: str) -> List[str]:
+    return spec[which]() if callable(spec[which]) else spec[which]
+
+
 _HEADERS = ["common.cuh"]
 _loaded: Dict[str, ctypes.CDLL] = {}
+_modules: Dict[str, object] = {}
 _lock = threading.Lock()
 
 
@@ -180,10 +205,11 @@ def build_library(name: str, verbose: bool = True) -> str:
     out_dir = build_dir()
     srcs = [os.path.join(CSRC, s) for s in spec["sources"]]
     hdrs = [os.path.join(CSRC, h) for h in _HEADERS + spec.get("deps", [])]
-    flags = ARCH_FLAGS + COMMON_FLAGS + spec["flags"]
+    flags = ARCH_FLAGS + COMMON_FLAGS + _flags(spec, "flags")
+    link = _flags(spec, "link")
     so = os.path.join(out_dir, library_file(name))
     stamp = so + ".stamp"
-    digest = _digest(srcs + hdrs, flags + spec["link"])
+    digest = _digest(srcs + hdrs, flags + link)
     if os.path.exists(so) and os.path.exists(stamp):
         with open(stamp) as f:
             if f.read().strip() == digest:
@@ -202,7 +228,7 @@ def build_library(name: str, verbose: bool = True) -> str:
     try:
         _run_with_heartbeat(cmds, f"'{name}'")
         tmp_so = f"{so}.{os.getpid()}.tmp"
-        _run_with_heartbeat([[nvcc] + ARCH_FLAGS + ["-shared", "-o", tmp_so] + objs + spec["link"]], f"'{name}' (link)")
+        _run_with_heartbeat([[nvcc] + ARCH_FLAGS + ["-shared", "-o", tmp_so] + objs + link], f"'{name}' (link)")
         os.replace(tmp_so, so)
         with open(stamp + f".{os.getpid()}", "w") as f:
             f.write(digest)
@@ -224,6 +250,19 @@ def load_library(name: str) -> ctypes.CDLL:
             lib = ctypes.CDLL(build_library(name))
             _loaded[name] = lib
         return lib
+
+
+def load_extension(name: str):
+    """The extension module ``name``, compiled first if need be."""
+    from importlib.machinery import ExtensionFileLoader
+    from importlib.util import module_from_spec, spec_from_loader
+    with _lock:
+        module = _modules.get(name)
+        if module is None:
+            module = module_from_spec(spec_from_loader(name, ExtensionFileLoader(name, build_library(name))))
+            module.__spec__.loader.exec_module(module)
+            _modules[name] = module
+        return module
 
 
 def build_all(verbose: bool = True) -> List[str]:

@@ -6,7 +6,8 @@ product), or one for each block of 128 x 128 of a weight.  A value stands for ``
 a block and a = max(amax, 448 * 2^-126), scale = a / 448 and q = round(x * (448 / a)), ties to even; a row's or a weight's last
 blocks may be partial.  What is not a number makes its block's scale not a number, an infinite value makes it infinite.
 
-Outputs are made when they are not given, and returned.  Given ones are contiguous, on the inputs' device, and overlap no input
+Outputs are made when they are not given, and returned; a call that gives none goes through one step of compiled code
+(fp8_calls.cpp), any other through the checks here.  Given ones are contiguous, on the inputs' device, and overlap no input
 (but ``add_rmsnorm`` adds into its residual where asked to).  The engine launches the same exported functions from its C++ parts.
 """
 from __future__ import annotations
@@ -19,6 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import ops
+from .build import load_extension
 from .ops import KernelError, call, register_signatures
 
 register_signatures("fp8", {
@@ -59,6 +61,31 @@ def _stream(what: str, first: torch.Tensor, *others) -> int:
     return ops._stream_now if ops._stream_now is not None else _raw_stream(at)
 
 
+_calls = None
+
+
+def _load_calls():
+    """The extension that makes a plain call in one step (fp8_calls.cpp), with the launchers it needs."""
+    global _calls
+    calls = load_extension("fp8_calls")
+    calls.set_launchers(*(ctypes.cast(ops._fn("fp8", f"ph_{n}")[0], c_void_p).value
+                          for n in ("quantize_fp8", "add_rmsnorm_fp8", "gated_fp8", "gemm_fp8_plan", "gemm_fp8")))
+    _calls = calls
+    return calls
+
+
+def _scope() -> int:
+    return -1 if ops._stream_now is None else ops._stream_now
+
+
+def _made(got):
+    """What a plain call gave: its outputs, or the status of a launcher that refused."""
+    if got.__class__ is int:
+        raise KernelError(ops._fn("fp8", "ph_quantize_fp8")[1]().decode("utf-8", "replace"))
+    ops.launches += 1
+    return got
+
+
 def _check(what: str, name: str, t: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
     """The output `name` that the caller has given."""
     if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
@@ -80,6 +107,10 @@ def quantize(x: torch.Tensor, out: Optional[torch.Tensor] = None, scales: Option
              block_rows: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [T, K] (float32 or bfloat16, its rows ``x.stride(0)`` apart) in 8 bits: out [T, K] and scales [ceil(T / block_rows),
     ceil(K / 128)].  ``block_rows``: 1 for the rows of a product, 128 for a weight."""
+    if out is None and scales is None:
+        got = (_calls or _load_calls()).quantize(x, block_rows, _scope())
+        if got is not None:
+            return _made(got)
     T, K = _matrix("quantize", "x", x)
     if block_rows not in (1, BLOCK):
         raise KernelError(f"quantize: block_rows is 1 or {BLOCK}, not {block_rows}")
@@ -104,6 +135,10 @@ def add_rmsnorm(x: torch.Tensor, add: Optional[torch.Tensor], weight: torch.Tens
     None), ``weight`` float32 [E].  v is kept in ``x_out`` [T, E] where that is given, else in x itself (unless ``write_x`` is
     false or there is nothing to add).  ``rows`` (int32 [n]) picks the rows that are normed, in that order (out [n, E]); nothing is
     kept then, and a number outside 0 .. T - 1 leaves its row of out and scales as it was."""
+    if out is None and scales is None and rows is None:
+        got = (_calls or _load_calls()).add_rmsnorm(x, add, weight, eps, add_splits, write_x, x_out, _scope())
+        if got is not None:
+            return _made(got)
     T, E = _matrix("add_rmsnorm", "x", x)
     if E > MAX_NORM_WIDTH:
         raise KernelError(f"add_rmsnorm: rows of at most {MAX_NORM_WIDTH} values, not {E}")
@@ -151,6 +186,10 @@ def gated(gate_up: torch.Tensor, out: Optional[torch.Tensor] = None, scales: Opt
     """out, scales = silu(g) * u in 8 bits for rows [g0, u0, g1, u1, ...]: gate_up [T, 2 F], or [splits, T, 2 F] partial sums
     with ``splits`` > 1 (float32 or bfloat16), to out [T, F], scales [T, ceil(F / 128)].  ``gate``: None (silu), (alpha, limit,
     shift) of the clamped swish, or "gelu_tanh"."""
+    if out is None and scales is None and gate is None:
+        got = (_calls or _load_calls()).gated(gate_up, splits, _scope())
+        if got is not None:
+            return _made(got)
     shape = gate_up.shape
     if len(shape) != (2 if splits == 1 else 3) or shape[-1] % 2 or not 0 < shape[-1] <= _LIMIT or splits < 1 or (splits > 1 and shape[0] != splits) or \
             not gate_up.is_contiguous():
@@ -191,6 +230,10 @@ def gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: tor
     choice): 16, 32 or 64 tokens beside 128 features, or 256 x 256 on pairs of CTAs.  ``early_w``: w is not the result of a
     kernel that may still run when the product starts (a model's weight), so its first tiles may be read before the kernel in
     front has ended."""
+    if out is None and not tile and not splits and (out_dtype is torch.bfloat16 or out_dtype is F32):
+        got = (_calls or _load_calls()).gemm(x, x_scales, w, w_scales, out_dtype is torch.bfloat16, early_w, _scope())
+        if got is not None:
+            return _made(got)
     M, K = _matrix("gemm_fp8", "x", x)
     N, K2 = _matrix("gemm_fp8", "w", w)
     if x.dtype is not E4M3 or w.dtype is not E4M3 or not x.is_contiguous() or not w.is_contiguous():

@@ -412,3 +412,34 @@ def test_feed_forward_in_graphs_and_streams():
         for j in range(2):
             assert torch.equal(graphs[j][1], want[i + j])
     fp8.check_errors()
+
+
+def test_plain_calls_and_checked_ones_are_the_same():
+    """A call without outputs takes the compiled step, one with them the checks of the face: the same launches."""
+    from purhie_b200.csrc import fp8, ops
+    x, a, w, gu = rnd(9, 264, seed=1), rnd(2, 9, 264, seed=2), 1 + 0.1 * rnd(264, seed=3), rnd(9, 528, seed=4).to(torch.bfloat16)
+
+    def outs(t, k, rows=1):
+        return torch.empty(t, k, device=DEV).to(torch.float8_e4m3fn), torch.empty(kblocks(t) if rows > 1 else t, kblocks(k), device=DEV)
+
+    def same(p, q):
+        return torch.equal(p[0].view(torch.uint8), q[0].view(torch.uint8)) and torch.equal(p[1], q[1])
+    before = ops.launches
+    for rows in (1, 128):
+        assert same(fp8.quantize(x, block_rows=rows), fp8.quantize(x, *outs(9, 264, rows), block_rows=rows))
+    assert same(fp8.gated(gu), fp8.gated(gu, *outs(9, 264)))
+    for parts, add in ((2, a), (1, a[0]), (1, a[:1]), (1, None)):
+        y, z = x.clone(), x.clone()
+        assert same(fp8.add_rmsnorm(y, add, w, 1e-6, add_splits=parts), fp8.add_rmsnorm(z, add, w, 1e-6, *outs(9, 264), add_splits=parts))
+        assert torch.equal(y, z) and torch.equal(y, x) == (add is None)
+    assert ops.launches == before + 14
+    xq, xs, wq, ws = operands(9, 200, 2064, 5)
+    for dtype in DT.values():
+        assert torch.equal(fp8.gemm(xq, xs, wq, ws, out_dtype=dtype), fp8.gemm(xq, xs, wq, ws, torch.empty(9, 200, dtype=dtype, device=DEV)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), ops.on_current_stream():
+        with torch.cuda.stream(torch.cuda.default_stream()):
+            q = fp8.quantize(x)                      # the scope's stream is the side stream, whatever is current inside it
+    side.synchronize()
+    assert same(q, fp8.quantize(x))
