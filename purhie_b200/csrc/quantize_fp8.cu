@@ -168,7 +168,7 @@ __device__ __forceinline__ void finish_block(uint8_t* row, float* scale, bool li
     store_block<W>(row, k0, lane16, K, v, TOP / a);
 }
 
-constexpr int ROW_THREADS = 256;
+constexpr int ROW_THREADS = 128;      // (2,048 rows of 12,288 gated values: 23.2 us; CTAs of 256 threads 24.0, of 512 27.3, of 64 23.1, but few rows 25 % longer)
 
 // U neighbouring blocks of rows for each half warp, all of them asked for before the first is worked on.
 template <typename T, int W, int U>
@@ -419,14 +419,14 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
 // Blocks for each half warp where they are many: what a lane holds while it waits is the same for both types.
 template <typename T> constexpr int MANY = 8 / (int)sizeof(T);
 
-// The number of blocks and of CTAs for them.  Several blocks a half warp once every SM has twice its fill of threads, else one: 2,048
-// rows of 12,288 gated bfloat16 values take 24.0 us with four, 29.9 with one and 34.7 with eight (and 26.7 where as many CTAs as the device holds walk over the blocks);
-// 256 such rows 6.5 and 5.5.
+// The number of blocks and of CTAs for them.  Several blocks a half warp once every SM has 256 blocks, else one: 2,048 rows of
+// 12,288 gated bfloat16 values take 23.2 us with four, 25.2 with two and 34.7 with eight (and 26.7 where as many CTAs as the device
+// holds walk over the blocks); 256 such rows 6.5 with four and 5.5 with one.
 inline bool count_blocks(long long rows, int width, int many, unsigned* blocks, int* u, unsigned* ctas) {
     const long long n = rows * ((width + BLOCK - 1) / BLOCK);
     if (n > 0x7fffffffLL - 4 * ROW_THREADS) return false;
     *blocks = (unsigned)n;
-    *u = n >= (long long)multiprocessors() * 16 * (ROW_THREADS / 16) ? many : 1;
+    *u = n >= (long long)multiprocessors() * 256 ? many : 1;
     *ctas = (unsigned)((n + (ROW_THREADS / 16) * *u - 1) / ((ROW_THREADS / 16) * *u));
     return true;
 }
