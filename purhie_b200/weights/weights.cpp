@@ -106,6 +106,9 @@ Tensor FolderSource::fetch(const std::string& name) {
                                    cudaMemcpyHostToDevice));
             }
         }
+        // A copy from memory that is not pinned returns once the last of it is staged; whoever works on the tensor in stream_, which
+        // does not wait for the default stream, must find all of it.
+        QE_CUDA(cudaStreamSynchronize(nullptr));
     }
     cache_[name] = t;
     return t;

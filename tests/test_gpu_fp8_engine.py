@@ -184,6 +184,23 @@ def test_feed_forward_part_is_the_faces_one_after_the_other(T, activation, gate,
     assert same
 
 
+def test_weights_are_whole_before_they_are_brought_to_8_bits(tmp_path):
+    """A matrix of a little more than 1 MiB: a copy from a file's mapping may return before its end is on the device."""
+    E, F = 272, 2048
+    x = torch.randn(9, E, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).float().numpy()
+    got = []
+    for i in range(8):
+        (tmp_path / str(i)).mkdir()
+        probe, _ = feed_forward_probe(tmp_path / str(i), E, F, None, {"gemm": "fp8"})
+        got.append(probe.feed_forward(x))
+    plain, _ = feed_forward_probe(tmp_path, E, F, None, {"gemm": "auto"})
+    want = plain.feed_forward(x)
+    for g in got:
+        assert np.array_equal(g, got[0])
+        # the last block of features, which the end of the matrix holds, is as near as all of them
+        assert np.linalg.norm((g - want)[:, 256:]) < 0.1 * np.linalg.norm(want[:, 256:])
+
+
 def test_matrices_that_do_not_fit_stay_as_they_are(tmp_path):
     """Rows of a number of values that is no multiple of 16 stay in bfloat16: the same bits as without the option."""
     E, F = 264, 656
