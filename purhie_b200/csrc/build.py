@@ -62,7 +62,7 @@ LIBRARIES: Dict[str, dict] = {
     },
     "fp8": {
         "sources": ["quantize_fp8.cu", "gemm_fp8.cu"],
-        "deps": ["mbarrier.cuh", "shared_limit.cuh"],
+        "deps": ["mbarrier.cuh", "shared_limit.cuh", "fp8_values.cuh"],
         "flags": [],
         "link": [],
     },

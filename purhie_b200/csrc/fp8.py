@@ -31,6 +31,7 @@ register_signatures("fp8", {
     "ph_fp8_take_error": [c_void_p],
     "ph_gemm_fp8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
                     c_void_p],
+    "ph_gemm_fp8_gated": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
     "ph_gemm_fp8_plan": [c_int, c_int, c_int, c_int, c_void_p, c_void_p],
 })
 
@@ -267,3 +268,27 @@ def gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: tor
     call("fp8", "ph_gemm_fp8", x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), whole, code, M, N, K, tile, splits, parts,
          early_w, None, stream)
     return out
+
+
+def gemm_gated(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: Optional[torch.Tensor] = None,
+               scales: Optional[torch.Tensor] = None, *, gate=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What ``gated`` makes of ``gemm``'s float32 product, without the product going to memory: w [N, K] holds the rows of gate and up in
+    turn (N a multiple of 256, K of 16), out [M, N / 2], scales [M, N / 256]; ``gate`` as in ``gated``.  For many tokens: it runs on
+    pairs of CTAs with K whole, whatever M is."""
+    M, K = _matrix("gemm_gated", "x", x)
+    N, K2 = _matrix("gemm_gated", "w", w)
+    if x.dtype is not E4M3 or w.dtype is not E4M3 or not x.is_contiguous() or not w.is_contiguous():
+        raise KernelError("gemm_gated: x and w must be contiguous float8_e4m3fn tensors")
+    kb = _blocks(K)
+    if K != K2 or N < 1 or N % 256:
+        raise KernelError(f"gemm_gated: x {tuple(x.shape)} and w {tuple(w.shape)} do not fit, or w's rows are no multiple of 256")
+    for name, t, rows in (("x_scales", x_scales, M), ("w_scales", w_scales, N // BLOCK)):
+        if t.dtype is not F32 or t.shape != (rows, kb) or not t.is_contiguous():
+            raise KernelError(f"gemm_gated: {name} must be contiguous float32 [{rows}, {kb}]")
+    stream = _stream("gemm_gated", x, x_scales, w, w_scales, out, scales)
+    out = _empty((M, N // 2), (N // 2, 1), dtype=E4M3, device=x.device) if out is None else _check("gemm_gated", "out", out, (M, N // 2), E4M3)
+    blocks = (M, N // 256)
+    scales = _empty(blocks, (blocks[1], 1), dtype=F32, device=x.device) if scales is None else _check("gemm_gated", "scales", scales, blocks, F32)
+    call("fp8", "ph_gemm_fp8_gated", x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), scales.data_ptr(), M, N, K,
+         _gate(gate), None, stream)
+    return out, scales

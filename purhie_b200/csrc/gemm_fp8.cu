@@ -15,12 +15,13 @@
 // (the norm and the activation take them), or a short kernel behind this one; the same bits every time.  (Cut among the CTAs of
 // a cluster that add up in shared memory, 8 x 6144 x 4096 took 16 us: a cluster starts late and not under the kernel in front.
 // With mma.sync and 16 features a CTA, K whole, 8 x 24576 x 4096 took 25 us: its 8-bit products are slow here.)
-// Many tokens: pairs of CTAs, further down.
+// Many tokens: pairs of CTAs, further down; theirs can end in a gated activation.
 //
 // Every wait on an mbarrier is bounded; a wait that runs out sets *error_flag, and the CTA still frees its tensor memory and
 // returns (what it writes is then meaningless).
 // The reference's counterpart is its WMMA tile kernel over 8-bit blocks (src/matvec_q.hip:3437-3547).
 #include "common.cuh"
+#include "fp8_values.cuh"
 #include "mbarrier.cuh"
 #include "shared_limit.cuh"
 
@@ -61,6 +62,9 @@ struct Params {
     int kblocks;
     int a_tiles, splits;
     int early_w;
+    // Pairs, the gated activation in the epilogue: w's rows are (gate, up) pairs, out is [M, N / 2] in e4m3 with out_scales [M, N / 256]
+    float* out_scales;
+    ph_fp8::Gate gate;
     int tma_store;               // pairs: the copy engine stores; 0: the threads do
     int* error_flag;
 };
@@ -427,6 +431,42 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
     return *(const uint32_t*)&h;
 }
 
+// A thread's 128 columns of its row as 64 gated values in 8 bits.  largest [turn][half][row of the CTA]: two turns, so that a warp that
+// is a tile ahead does not write what its partner has yet to read.  Tiles are whole (N a multiple of 256).
+__device__ __forceinline__ void store_gated(const Params& p, float* acc, float* largest, int turn, int q, int half, int lane, int row, int n0) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < PAIR_HALF / 2; ++j) {
+        acc[j] = ph_fp8::gated_value(p.gate, acc[2 * j], acc[2 * j + 1]);
+        m = ph_fp8::max_nan(m, fabsf(acc[j]));
+    }
+    float* at = largest + turn * 2 * BM + q * 32 + lane;
+    at[half * BM] = m;
+    asm volatile("bar.sync %0, 64;" ::"r"(2 + q) : "memory");
+    const float a = ph_fp8::max_nan(ph_fp8::max_nan(m, at[(half ^ 1) * BM]), ph_fp8::LEAST);
+    if (row >= p.M) return;
+    const int F = p.N / 2;
+    if (half == 0) p.out_scales[(size_t)row * (F / ph_fp8::BLOCK) + n0 / PAIR_BN] = a / ph_fp8::TOP;
+    const float inverse = ph_fp8::TOP / a;
+    uint4* o = (uint4*)((uint8_t*)p.out + (size_t)row * F + n0 / 2);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* h = acc + c * 16 + i * 4;
+            v[i] = ph_fp8::pack2(h[0] * inverse, h[1] * inverse) | ph_fp8::pack2(h[2] * inverse, h[3] * inverse) << 16;
+        }
+        o[c] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+// GATED: the epilogue applies the gated activation and brings its values to 8 bits.  A tile's 256 features are 128 (gate, up) pairs, one
+// block of the result for each of its rows: the two warps that hold a row's halves tell each other their largest magnitudes.  The tensor
+// cores stand still while a tile's 64 exponentials a thread are made (2048 x 24576 x 4096: 244 us, 217 and 25 as two kernels; 8192 rows
+// 876, 825 and 97), but the product's 100 MB neither leave nor come back: a prompt of 2,048 tokens through 36 such layers, at the power
+// limit, takes 22.7 ms for 23.25.
+template <bool GATED>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out, Params p) {
     constexpr int STAGES = PAIR_STAGES;
@@ -564,6 +604,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PAIR_REGS_HIGH));
         const int q = warp & 3, half = (warp - 4) >> 2;               // rows 32 q .. 32 q + 31, columns 128 half .. 128 half + 127
         uint8_t* boxes = staging + (warp - 4) * 2 * PAIR_BOX_BYTES;
+        int turn = 0;
         int buf = 0;
         uint32_t buf_phase = 0;
         bool ok = true;
@@ -596,7 +637,6 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             part_of_k(i, kb0, blocks);
             blocks -= kb0;
             const int row0 = (t % a_tiles) * 2 * BM + (int)rank * BM + q * 32, n0 = (t / a_tiles) * PAIR_BN + half * PAIR_HALF;
-            const int row = row0 + lane;
             float acc[PAIR_HALF];
 #pragma unroll
             for (int j = 0; j < PAIR_HALF; ++j) acc[j] = 0.0f;
@@ -624,7 +664,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                 }
                 f = f_next;
             }
-            if (row0 >= p.M || n0 >= p.N) continue;                   // the whole warp
+            if (row0 >= p.M || (!GATED && n0 >= p.N)) continue;       // the whole warp (with the activation, both of a row's)
+            if constexpr (GATED) {
+                store_gated(p, acc, (float*)staging, turn, q, half, lane, row0 + lane, n0);
+                turn ^= 1;
+                continue;
+            }
             // Boxes of 32 rows x 128 bytes, swizzled as the copy engine wants them (16-byte chunk ^ (row & 7)).  It stores them, and leaves
             // out what lies outside of out; rows that do not start on 16 bytes (an odd width) are stored by the warp, a row at a time
             // (3666 x 22705 x 432: 860 us where every thread stored its own row, value by value).
@@ -726,14 +771,15 @@ bool make_out_map(CUtensorMap* out, const void* ptr, bool bf16, int parts, int r
 }
 
 int launch_pair(const void* x, const void* w, Params p, int K, cudaStream_t stream) {
-    if (const int rc = allow_shared<gemm_fp8_pair_kernel>(PAIR_SMEM_BYTES, "gemm_fp8_pair")) return rc;
+    const bool gated = p.out_scales != nullptr;
+    if (const int rc = gated ? allow_shared<gemm_fp8_pair_kernel<true>>(PAIR_SMEM_BYTES, "gemm_fp8_pair") : allow_shared<gemm_fp8_pair_kernel<false>>(PAIR_SMEM_BYTES, "gemm_fp8_pair")) return rc;
     CUtensorMap ma, mb, mo;
     if (!make_map(&ma, x, p.M, K, BM) || !make_map(&mb, w, p.N, K, PAIR_HALF))
         return fail(PH_ERR_LAUNCH, "gemm_fp8_pair: cuTensorMapEncodeTiled failed (M %d, N %d, K %d)", p.M, p.N, K);
     // the copy engine stores where its rules allow: rows of a multiple of 16 bytes on 16-byte boundaries
     mo = ma;
     p.tma_store = 0;
-    if ((p.N * (p.out_bf16 ? 2LL : 4LL)) % 16 == 0 && ((uintptr_t)p.out & 15) == 0 && make_out_map(&mo, p.out, p.out_bf16, p.splits, p.M, p.N)) p.tma_store = 1;
+    if (!gated && (p.N * (p.out_bf16 ? 2LL : 4LL)) % 16 == 0 && ((uintptr_t)p.out & 15) == 0 && make_out_map(&mo, p.out, p.out_bf16, p.splits, p.M, p.N)) p.tma_store = 1;
     p.a_tiles = (p.M + 2 * BM - 1) / (2 * BM);
     const long long tiles = (long long)p.a_tiles * ((p.N + PAIR_BN - 1) / PAIR_BN) * p.splits;
     if (tiles > 0x3fffffffLL) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8_pair: %d x %d has too many tiles", p.M, p.N);
@@ -748,7 +794,7 @@ int launch_pair(const void* x, const void* w, Params p, int K, cudaStream_t stre
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, gemm_fp8_pair_kernel, ma, mb, mo, p);
+    cudaLaunchKernelEx(&cfg, gated ? gemm_fp8_pair_kernel<true> : gemm_fp8_pair_kernel<false>, ma, mb, mo, p);
     return check_launch("gemm_fp8_pair");
 }
 
@@ -842,6 +888,24 @@ PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const f
     if (out_dtype == PH_BF16) launch_overlapped(sum_parts_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)parts, splits, values, (__nv_bfloat16*)out);
     else launch_overlapped(sum_parts_kernel<float>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)parts, splits, values, (float*)out);
     return check_launch("gemm_fp8 (sum of the parts)");
+}
+
+// The product of (gate, up) rows with the gated activation behind it, in 8 bits: w [N, K] holds the rows of gate and up in turn, q [M, N / 2] and
+// scales [M, N / 256] what ph_gated_fp8 would make of the float32 product (which never leaves the SMs).  On pairs of CTAs, K whole; N a multiple of 256.
+// gate: as ph_gated_fp8's.
+PH_EXPORT int ph_gemm_fp8_gated(const void* x, const float* xs, const void* w, const float* ws, void* q, float* scales, int M, int N, int K, const float* gate, int* error_flag,
+                                cudaStream_t stream) {
+    if (M == 0) return PH_OK;
+    if (!x || !xs || !w || !ws || !q || !scales || M < 1 || N < 1 || K < 1) return fail(PH_ERR_ARG, "gemm_fp8_gated: bad arguments (M %d, N %d, K %d)", M, N, K);
+    if (M > MAX_SIZE || N > MAX_SIZE || K > MAX_SIZE) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8_gated: M, N and K of at most %d, not %d, %d and %d", MAX_SIZE, M, N, K);
+    if (K % 16 || N % PAIR_BN) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8_gated: K = %d must be a multiple of 16 and N = %d one of %d", K, N, PAIR_BN);
+    if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)q) & 15) return fail(PH_ERR_UNSUPPORTED, "gemm_fp8_gated: operands and q must be 16-byte aligned");
+    Params p = {};
+    p.xs = xs; p.ws = ws; p.M = M; p.N = N; p.kblocks = (K + BK - 1) / BK; p.splits = 1; p.error_flag = error_flag; p.out = q; p.out_scales = scales;
+    p.gate = ph_fp8::Gate{0, 1.0f, 0.0f, 0.0f};
+    if (gate) p.gate = ph_fp8::Gate{(int)gate[3], gate[0], gate[1], gate[2]};
+    if (p.gate.kind < 0 || p.gate.kind > 2) return fail(PH_ERR_ARG, "gemm_fp8_gated: gate %d is not known", p.gate.kind);
+    return launch_pair(x, w, p, K, stream);
 }
 
 // The number that a wait which ran out has left on the current device since the last call (0: none); waits for the device.

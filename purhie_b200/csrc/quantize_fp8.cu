@@ -14,42 +14,20 @@
 // memory: each input is read once and held in registers until its block's scale is known.
 // The reference's counterpart is its 8-bit activation blocks (src/matvec_q.hip), whose scales are per 32 values.
 #include "common.cuh"
+#include "fp8_values.cuh"
 #include "shared_limit.cuh"
-
-#include <cuda_fp8.h>
 
 namespace {
 
 using namespace ph;
+using namespace ph_fp8;
 
-constexpr int BLOCK = 128;
 constexpr int MAX_WIDTH = 1 << 30;                             // of a row: its blocks are counted in 32 bits
-constexpr float TOP = 448.0f;                                  // the largest e4m3 value
-constexpr float LEAST = 448.0f * 1.17549435e-38f;              // 448 * 2^-126
-
-// max and min that keep what is no number
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 // The largest magnitude over the 16 lanes that share a block.
 __device__ __forceinline__ float half_warp_max(float v) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
-}
-
-// Two values to e4m3, the first in the low byte.
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 
 // The place of a lane's value i inside its block, for vectors of W values.
@@ -304,21 +282,6 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(NormParams p) {
         for (int i = 0; i < 8; ++i) y.v[i] = v[u][i] * f * w[i];
         finish_block<W>(p.q + r * p.E, p.scales + r * p.kblocks + b, b < p.kblocks, b * BLOCK, lane16, p.E, y);
     }
-}
-
-// The gated activation of a (gate, up) pair.  kind 0: silu(g) * u; 1 clamped swish: g' = min(g, limit), u' = clamp(u, -limit,
-// limit), g' * sigmoid(alpha g') * (u' + shift); 2: gelu(g) * u in the tanh form, 0.5 g (1 + tanh(y)) = g sigmoid(2 y),
-// y = sqrt(2/pi) (g + 0.044715 g^3).
-struct Gate {
-    int kind;
-    float alpha, limit, shift;
-};
-__device__ __forceinline__ float gated_value(const Gate& gate, float g, float u) {
-    if (gate.kind == 0) return __fdividef(g, 1.0f + __expf(-g)) * u;
-    if (gate.kind == 2) return __fdividef(g, 1.0f + __expf(-1.5957691216057308f * (g + 0.044715f * g * g * g))) * u;
-    g = min_nan(g, gate.limit);
-    u = min_nan(max_nan(u, -gate.limit), gate.limit);
-    return __fdividef(g, 1.0f + __expf(-gate.alpha * g)) * (u + gate.shift);
 }
 
 // Rows of (g0, u0, g1, u1, ...), in `parts` parts that are summed first, to gated rows of F in 8 bits; U blocks for each half warp.

@@ -303,6 +303,7 @@ const Fp8Kernels& fp8_kernels() {
     bind(h, "fp8", "ph_add_rmsnorm_fp8", g_fp8.add_rmsnorm);
     bind(h, "fp8", "ph_gated_fp8", g_fp8.gated);
     bind(h, "fp8", "ph_gemm_fp8_plan", g_fp8.plan);
+    bind(h, "fp8", "ph_gemm_fp8_gated", g_fp8.gemm_gated);
     bind(h, "fp8", "ph_gemm_fp8", g_fp8.gemm);
     bind(h, "fp8", "ph_fp8_last_error", g_fp8.last_error);
     g_fp8_ok = true;

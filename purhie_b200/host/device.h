@@ -303,6 +303,7 @@ struct Fp8Kernels {
     int (*add_rmsnorm)(const float*, const void*, int, int, long long, const float*, float, const int32_t*, int, int, int, float*, void*, float*,
                        cudaStream_t);
     int (*gated)(const void*, int, int, long long, void*, float*, int, int, const float*, cudaStream_t);
+    int (*gemm_gated)(const void*, const float*, const void*, const float*, void*, float*, int, int, int, const float*, int*, cudaStream_t);
     int (*plan)(int, int, int, int, int*, int*);
     int (*gemm)(const void*, const float*, const void*, const float*, void*, int, int, int, int, int, int, float*, int, int*, cudaStream_t);
     const char* (*last_error)(void);

@@ -68,6 +68,14 @@ public:
         // where the tensor-core product runs, its epilogue applies the gate (either family); else a kernel behind it does
         float gate_constants[4];
         gate_.constants(gate_constants);
+        if (down_.eight_bit()) {
+            // many rows in 8 bits: the first product's epilogue gives the second one's rows
+            Tensor scales, act8 = gate_up_.gated_eight_bit(x, ctx, "ff_act8", T, gate_.kind ? gate_constants : nullptr, &scales);
+            if (act8.defined()) {
+                ctx.row8_scales = scales.as<float>();
+                return down_(act8, ctx, "ff_out", DType::F32, T, true, false, ctx.residual, nullptr, &ctx.norm_ahead);
+            }
+        }
         Addend gu = gate_up_(x, ctx, "gate_up", compute_dtype, T, true, true, nullptr, &ctx.row_scale, nullptr,
                              gate_.kind ? gate_constants : nullptr);
         Tensor act;

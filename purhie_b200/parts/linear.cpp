@@ -136,20 +136,44 @@ Linear Linear::first_features(int64_t n, std::string label, const std::string& g
     return l;
 }
 
+const void* Linear::eight_bit_rows(const Tensor& x, StepContext& ctx, int M, const float** row_scales) const {
+    const int K = (int)weight_.shape[1], kb = ceil_div(K, kScaleBlock);
+    if (x.dtype == DType::U8) {
+        if (!ctx.row8_scales) throw Error(kInvalidState, label_ + ": rows in 8 bits came without their scales");
+        *row_scales = ctx.row8_scales;
+        return x.data;
+    }
+    const Fp8Kernels& k = fp8_kernels();
+    Tensor q = ctx.workspace->get("linear_rows8", {M, K}, DType::U8), s = ctx.workspace->get("linear_rows8_scales", {M, kb}, DType::F32);
+    if (LaunchProfile::get().on()) LaunchProfile::get().note_cost((double)M * K * (dtype_size(x.dtype) + 1) + 4.0 * M * kb, 0.0);
+    QE_LAUNCH(k, k.quantize(x.data, x.code(), K, q.data, s.as<float>(), M, K, 1, ctx.stream));
+    *row_scales = s.as<float>();
+    return q.data;
+}
+
+Tensor Linear::gated_eight_bit(const Tensor& x, StepContext& ctx, const std::string& out_name, int rows, const float* gate, Tensor* scales) const {
+    constexpr int kPairTile = 256;           // of the kernel on pairs of CTAs, which alone has the activation
+    const int M = rows, N = (int)weight_.shape[0], K = (int)weight_.shape[1];
+    if (!eight_bit() || N % kPairTile) return Tensor();
+    const Fp8Kernels& k = fp8_kernels();
+    int tile = 0, splits = 0;
+    if (k.plan(M, N, K, 0, &tile, &splits) != 0) throw KernelError(k.last_error());
+    if (tile != kPairTile || splits != 1) return Tensor();
+    const float* row_scales = nullptr;
+    const void* q = eight_bit_rows(x, ctx, M, &row_scales);
+    Tensor out = ctx.workspace->get(out_name, {M, N / 2}, DType::U8);
+    *scales = ctx.workspace->get(out_name + "_scales", {M, N / kPairTile}, DType::F32);
+    if (LaunchProfile::get().on()) LaunchProfile::get().note_cost((double)N * K + (double)M * K + (double)M * N / 2, 2.0 * M * N * K);
+    QE_LAUNCH(k, k.gemm_gated(q, row_scales, weight_.data, scales_.as<float>(), out.data, scales->as<float>(), M, N, K, gate, ctx.gemm_error, ctx.stream));
+    return out;
+}
+
 Addend Linear::eight_bit_product(const Tensor& x, StepContext& ctx, const std::string& out_name, DType out_dtype, int M, bool allow_split, void* into) const {
-    const int N = (int)weight_.shape[0], K = (int)weight_.shape[1], kb = ceil_div(K, kScaleBlock);
+    const int N = (int)weight_.shape[0], K = (int)weight_.shape[1];
     const Fp8Kernels& k = fp8_kernels();
     Workspace& ws = *ctx.workspace;
-    const void* rows = x.data;
-    const float* row_scales = ctx.row8_scales;
-    if (x.dtype != DType::U8) {
-        Tensor q = ws.get("linear_rows8", {M, K}, DType::U8), s = ws.get("linear_rows8_scales", {M, kb}, DType::F32);
-        if (LaunchProfile::get().on()) LaunchProfile::get().note_cost((double)M * K * (dtype_size(x.dtype) + 1) + 4.0 * M * kb, 0.0);
-        QE_LAUNCH(k, k.quantize(x.data, x.code(), K, q.data, s.as<float>(), M, K, 1, ctx.stream));
-        rows = q.data;
-        row_scales = s.as<float>();
-    }
-    if (!row_scales) throw Error(kInvalidState, label_ + ": rows in 8 bits came without their scales");
+    const float* row_scales = nullptr;
+    const void* rows = eight_bit_rows(x, ctx, M, &row_scales);
     int tile = 0, splits = 0;
     if (k.plan(M, N, K, allow_split ? 0 : 1, &tile, &splits) != 0) throw KernelError(k.last_error());
     const bool hand_on = allow_split && splits > 1;          // whoever consumes the product adds the parts up

@@ -51,6 +51,9 @@ public:
     Addend operator()(const Tensor& x, StepContext& ctx, const std::string& out_name, DType out_dtype, int rows,
                       bool allow_split = false, bool fuse_swiglu = false, float* add_into = nullptr,
                       const RowScale* scale = nullptr, NormAhead* ahead = nullptr, const float* gate = nullptr) const;
+    // A weight of (gate, up) row pairs in 8 bits and many rows of x: the gated activation of the product in 8 bits, [rows, out / 2] with
+    // its scales in *scales, where the kernel that does both is the one for this size; else nothing is done and the tensor is undefined.
+    Tensor gated_eight_bit(const Tensor& x, StepContext& ctx, const std::string& out_name, int rows, const float* gate, Tensor* scales) const;
     // The plain product, K whole, written to `out` ([rows, out_features], any dtype the kernels write): for a caller
     // that lays several products' results out side by side (the experts of a routed feed-forward).
     void into(const Tensor& x, StepContext& ctx, Tensor out, int rows) const;
@@ -63,6 +66,8 @@ public:
     // Many rows, K cut into parts: float32 partial sums, linear in the rows, so whoever adds them up can apply the factor.
     bool gives_partial_sums(int rows, bool allow_split) const;
 private:
+    // x's rows in 8 bits and their scales: as they came, or made here
+    const void* eight_bit_rows(const Tensor& x, StepContext& ctx, int M, const float** row_scales) const;
     // [M, N] in out_dtype, or (parts wanted and better) float32 parts of it
     Addend eight_bit_product(const Tensor& x, StepContext& ctx, const std::string& out_name, DType out_dtype, int M, bool allow_split, void* out) const;
     Tensor weight_;          // eight_bit(): bytes, e4m3

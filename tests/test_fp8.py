@@ -53,6 +53,9 @@ REFUSED = [
     ("do not fit", lambda: fp8.gemm(e4m3(2, 64), f32(2, 1), e4m3(0, 64), f32(0, 1))),
     ("x_scales", lambda: fp8.gemm(e4m3(2, 144), f32(2, 1), e4m3(8, 144), f32(1, 2))),
     ("w_scales", lambda: fp8.gemm(e4m3(2, 144), f32(2, 2), e4m3(129, 144), f32(1, 2))),
+    ("multiple of 256", lambda: fp8.gemm_gated(e4m3(2, 64), f32(2, 1), e4m3(128, 64), f32(1, 1))),
+    ("w_scales", lambda: fp8.gemm_gated(e4m3(2, 64), f32(2, 1), e4m3(256, 64), f32(1, 1))),
+    ("CUDA", lambda: fp8.gemm_gated(e4m3(2, 64), f32(2, 1), e4m3(256, 64), f32(2, 1))),
     ("CUDA", lambda: fp8.gemm(e4m3(2, 64), f32(2, 1), e4m3(8, 64), f32(1, 1))),
 ]
 
@@ -89,6 +92,10 @@ C_REFUSED = [
     ("summed here", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 256, 16, 2, X + 4, 0, None, None)),
     ("parts of K", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 256, 16, 3, X, 0, None, None)),
     ("tile 128", "ph_gemm_fp8", (X, S, X, S, X, 0, 4, 8, 256, 128, 1, None, 0, None, None)),
+    ("one of 256", "ph_gemm_fp8_gated", (X, S, X, S, X, S, 4, 128, 32, None, None, None)),
+    ("multiple of 16", "ph_gemm_fp8_gated", (X, S, X, S, X, S, 4, 256, 24, None, None, None)),
+    ("aligned", "ph_gemm_fp8_gated", (X, S, X, S, X + 8, S, 4, 256, 32, None, None, None)),
+    ("gate 5", "ph_gemm_fp8_gated", (X, S, X, S, X, S, 4, 256, 32, (fp8.c_float * 4)(0, 0, 0, 5), None, None)),
     ("no plan", "ph_gemm_fp8_plan", (0, 8, 32, 1, X, S)),
     ("no plan", "ph_gemm_fp8_plan", (4, 8, 32, 1, None, S)),
 ]

@@ -312,6 +312,42 @@ def test_product_on_pairs(M, N, K, out):
     fp8.check_errors()
 
 
+@pytest.mark.parametrize("gate", [None, (1.702, 7.0, 1.0), "gelu_tanh"])
+@pytest.mark.parametrize("M,N,K", [(1, 256, 16), (255, 768, 272), (300, 512, 2064), (1000, 2304, 656), (2100, 5120, 400)])
+def test_product_with_the_activation(M, N, K, gate):
+    """The fused form is the product on pairs and the activation of its float32 values: more tiles than pairs and fewer, rows that end
+    inside a tile."""
+    from purhie_b200.csrc import fp8
+    x, xs, w, ws = operands(M, N, K, M + N + K)
+    xs *= 0.01
+    ws *= 0.01
+    y = fp8.gemm(x, xs, w, ws, out_dtype=torch.float32, tile=256, splits=1)
+    held_q, held_s = torch.full((M + 2, N // 2), 3.0, device=DEV).to(torch.float8_e4m3fn), torch.full((M + 2, N // 256), -1.0, device=DEV)
+    q, s = fp8.gemm_gated(x, xs, w, ws, held_q[1:M + 1], held_s[1:M + 1], gate=gate)
+    want_q, want_s = fp8.gated(y, gate=gate)
+    assert torch.equal(s, want_s) and torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
+    for i in (0, M + 1):
+        assert (held_q[i].float() == 3).all() and (held_s[i] == -1).all()
+    h, arg, num, up = gate_value(y[:, 0::2].double(), y[:, 1::2].double(), gate)
+    rel = (24 + 8 * arg.abs().clamp(max=90)) * U + (num * up).abs() * 2.0 ** -125 / h.abs().clamp(min=1e-300)
+    check_quantized(q, s, h, 1, rel)
+    fp8.check_errors()
+
+
+def test_product_with_the_activation_keeps_what_is_not_a_number():
+    from purhie_b200.csrc import fp8
+    x, xs, w, ws = operands(300, 512, 256, 1)
+    xs *= 0.01
+    ws *= 0.01
+    xs[7, 1] = float("nan")
+    xs[290, 0] = float("inf")
+    q, s = fp8.gemm_gated(x, xs, w, ws)
+    assert torch.isnan(s[7]).all() and not torch.isfinite(s[290]).any()
+    fine = torch.ones(300, dtype=torch.bool, device=DEV)
+    fine[7] = fine[290] = False
+    assert torch.isfinite(s[fine]).all() and torch.isfinite(q[fine].float()).all()
+
+
 def test_product_refusals():
     from purhie_b200.csrc import fp8
     from purhie_b200.native import KernelError

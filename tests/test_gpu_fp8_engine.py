@@ -157,13 +157,13 @@ def feed_forward_probe(tmp_path, E, F, activation, options):
     return probe, {k: v.to(DEV) for k, v in w.items()}
 
 
-@pytest.mark.parametrize("T", [1, 5, 40, 300, 700])
+@pytest.mark.parametrize("T,F", [(1, 656), (5, 656), (40, 656), (300, 656), (700, 656), (9, 2048), (600, 2048), (1500, 2048)])
 @pytest.mark.parametrize("activation,gate", [(None, None), ({"kind": "clamped_swish", "alpha": 1.7, "limit": 3.0, "shift": 1.0}, (1.7, 3.0, 1.0)),
                                              ({"kind": "gelu_tanh"}, "gelu_tanh")])
-def test_feed_forward_part_is_the_faces_one_after_the_other(T, activation, gate, tmp_path):
+def test_feed_forward_part_is_the_faces_one_after_the_other(T, F, activation, gate, tmp_path):
     """The part launches what the faces launch: the same bits."""
     from purhie_b200.csrc import fp8
-    E, F = 272, 656
+    E = 272
     probe, w = feed_forward_probe(tmp_path, E, F, activation, {"gemm": "fp8"})
     x = torch.randn(T, E, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
     got = torch.from_numpy(probe.feed_forward(x.float().numpy()))
@@ -175,8 +175,11 @@ def test_feed_forward_part_is_the_faces_one_after_the_other(T, activation, gate,
         # as the parts ask for it: the parts of K, where there are several, go to whoever reads them
         tile, splits = fp8.plan(q.shape[0], w.shape[0], w.shape[1], whole=False)
         return fp8.gemm(q, s, w, ws, tile=tile, splits=splits, out_dtype=dtype), splits
-    y, n = product(q, s, gu, gus, torch.bfloat16)
-    q2, s2 = fp8.gated(y, splits=n, gate=gate)
+    if F % 128 == 0 and fp8.plan(T, 2 * F, E) == (256, 1):
+        q2, s2 = fp8.gemm_gated(q, s, gu, gus, gate=gate)
+    else:
+        y, n = product(q, s, gu, gus, torch.bfloat16)
+        q2, s2 = fp8.gated(y, splits=n, gate=gate)
     out, n = product(q2, s2, dn, dns, torch.float32)
     if n > 1:
         out = out.double().sum(0).float()                            # the probe adds the parts up in double precision
