@@ -815,9 +815,11 @@ int launch(const void* x, const void* w, Params p, int K, cudaStream_t stream) {
 // The tile (16, 32 or 64 tokens beside 128 features; 256: pairs) and the parts of K with the least estimated time, among those that
 // the caller leaves open (0).  Microseconds: a launch (a pair's does not start early), rounds of the CTAs over the device's places
 // times (an item's start and end + its blocks of K), the weight's way from memory and the tiles' from L2, and for several parts
-// their way out and back and, where the whole sum is wanted, the kernel that adds them up.  Fitted to 1,538 launches at 1 to 2,048
+// their way out and back and the kernel that adds them up, or what they cost whoever consumes them.  Fitted to 1,538 launches at 1 to 2,048
 // tokens, 256 to 24,576 features and K 512 to 16,384 (root mean square error 5 %); what it picks takes 1.5 % longer than the
 // best of all, over those 80 products.  (Tiles of 128 tokens were never the best by more than 1 %, and are gone.)
+// Parts that are handed on cost their consumer 0.8 us and 0.1 us each: with that, one row through the products, norms and
+// quantizers of a layer of the 8B shape takes 46.5 us and not 48.3 (gate and up whole, not in three parts).
 void choose(int M, int N, int K, int sms, bool whole, int* tile, int* splits) {
     struct Kind { int tile, per_sm; double launch, item, block; };
     static const Kind kinds[] = {{16, 2, 0.26, 1.92, 0.339}, {32, 2, 0.26, 2.34, 0.358}, {64, 2, 0.26, 3.61, 0.404}, {256, 0, 4.08, 1.54, 0.491}};
@@ -833,7 +835,7 @@ void choose(int M, int N, int K, int sms, bool whole, int* tile, int* splits) {
             if (asked_splits != 0 && s != asked_splits) continue;
             const int blocks = (kblocks + s - 1) / s;
             double cost = k.launch + ceil(tiles * s / slots) * (k.item + k.block * blocks) + weight_mb / 28.2 + tiles * s * blocks * stage_mb / 51.7;
-            if (s > 1) cost += (whole ? 1.38 : 0.0) + 0.136 * s + s * 8e-6 * M * N / 9.8;
+            if (s > 1) cost += (whole ? 1.38 + 0.136 * s : 0.8 + 0.236 * s) + s * 8e-6 * M * N / 9.8;
             if (best < 0 || cost < best - 1e-9) { best = cost; *tile = k.tile; *splits = s; }
         }
     }

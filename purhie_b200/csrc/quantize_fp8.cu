@@ -208,7 +208,9 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
 }
 
 // v = x[t] + sum over the parts of add[s][t]; v to x_out[t] (or nowhere); y = v * rsqrt(mean(v^2) + eps) * weight to 8 bits.
-// One CTA a row, U blocks for each half warp.
+// One CTA a row, U blocks for each half warp.  AHEAD: how many parts are asked for at a time (they are added in their order); above 1
+// the weight comes before the row's sum too, and a line of it to L2 before the kernel in front is done.
+constexpr int ALONE = 6;             // the AHEAD of CTAs that have an SM for themselves, in the registers that this leaves
 struct NormParams {
     const float* x;
     const void* add;
@@ -223,11 +225,17 @@ struct NormParams {
     float* scales;
 };
 
-template <typename A, int W, int U>
-__global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(NormParams p) {
+template <typename A, int W, int U, int AHEAD>
+__global__ void __launch_bounds__(AHEAD == ALONE ? 640 : 1024) add_rmsnorm_fp8_kernel(NormParams p) {
+    constexpr bool MORE = AHEAD > 1;
     __shared__ float scratch[32];
     const int lane16 = threadIdx.x & 15, half = threadIdx.x >> 4, halves = blockDim.x >> 4;
     pdl_launch_dependents();
+#pragma unroll
+    for (int u = 0; u < (MORE ? U : 0); ++u) {
+        const int k = (half + u * halves) * BLOCK + lane16 * 8;
+        if (k < p.E) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.weight + k));
+    }
     pdl_wait();
     const long long r = blockIdx.x;
     const long long t = p.rows ? p.rows[r] : r;
@@ -238,15 +246,26 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(NormParams p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) load_block<W>(x, (half + u * halves) * BLOCK, lane16, p.E, v[u]);
     if (p.add) {
-        for (int s = 0; s < p.parts; ++s) {
+        for (int s = 0; s < p.parts; s += AHEAD) {
+            Held<A> a[AHEAD][U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float a[8];
-                load_block<W>(add + s * p.part_stride, (half + u * halves) * BLOCK, lane16, p.E, a);
+            for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] += a[i];
-            }
+                for (int u = 0; u < U; ++u)
+                    if (s + j < p.parts) hold_block<W>(add + (s + j) * p.part_stride, (half + u * halves) * BLOCK, lane16, p.E, a[j][u]);
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (s + j < p.parts) v[u][i] += a[j][u].get(i);
         }
+    }
+    float w[U][8];
+    if (MORE) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_block<W>(p.weight, (half + u * halves) * BLOCK, lane16, p.E, w[u]);
     }
     float ss = 0.0f;
 #pragma unroll
@@ -275,11 +294,10 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(NormParams p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int b = half + u * halves;
-        float w[8];
-        load_block<W>(p.weight, b * BLOCK, lane16, p.E, w);
+        if (!MORE) load_block<W>(p.weight, b * BLOCK, lane16, p.E, w[u]);
         Held<float> y;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y.v[i] = v[u][i] * f * w[i];
+        for (int i = 0; i < 8; ++i) y.v[i] = v[u][i] * f * w[u][i];
         finish_block<W>(p.q + r * p.E, p.scales + r * p.kblocks + b, b < p.kblocks, b * BLOCK, lane16, p.E, y);
     }
 }
@@ -352,12 +370,20 @@ __global__ void __launch_bounds__(ROW_THREADS) gated_fp8_kernel(const T* __restr
 #pragma unroll
             for (int i = 0; i < 16; ++i) g[i] = 0.0f;
             if (live && k0 + lane16 * 8 < F) {
-                for (int s = 0; s < parts; ++s) {
-                    float a[16];
-                    load8(src + s * part_stride + 2 * (k0 + lane16 * 8), a);
-                    load8(src + s * part_stride + 2 * (k0 + lane16 * 8) + 8, a + 8);
+                for (int s = 0; s < parts; s += 3) {                 // three at a time (8 rows of 12,288: 2.1 us, 2.2 one by one; 64 4.1 and 4.6)
+                    Held<T> a[3][2];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) g[i] = s == 0 ? a[i] : g[i] + a[i];
+                    for (int j = 0; j < 3; ++j)
+                        if (s + j < parts) {
+                            a[j][0].load(src + (s + j) * part_stride + 2 * (k0 + lane16 * 8));
+                            a[j][1].load(src + (s + j) * part_stride + 2 * (k0 + lane16 * 8) + 8);
+                        }
+#pragma unroll
+                    for (int j = 0; j < 3; ++j)
+                        if (s + j < parts) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) g[i] = s + j == 0 ? a[j][i >> 3].get(i & 7) : g[i] + a[j][i >> 3].get(i & 7);
+                        }
                 }
             }
 #pragma unroll
@@ -403,11 +429,12 @@ int launch_norm(const NormParams& p, int n, cudaStream_t stream) {
     const int u = p.kblocks <= 64 ? 1 : p.kblocks <= 128 ? 2 : 4;
     const int halves = (p.kblocks + u - 1) / u;
     const int threads = (halves * 16 + 31) / 32 * 32;
-    switch (u) {
-        case 1: launch_overlapped(add_rmsnorm_fp8_kernel<A, W, 1>, dim3(n), dim3(threads), 0, stream, p); break;
-        case 2: launch_overlapped(add_rmsnorm_fp8_kernel<A, W, 2>, dim3(n), dim3(threads), 0, stream, p); break;
-        default: launch_overlapped(add_rmsnorm_fp8_kernel<A, W, 4>, dim3(n), dim3(threads), 0, stream, p); break;
-    }
+    // Several parts come from few rows: one request behind the other, a row of 4,096 in nine of them took 3.7 us, four at a time 3.3.  Where
+    // every row has an SM for itself six are asked for (in a layer of an 8B shape behind its products, two norms of 64 rows 9.5 us with
+    // four, 6.0 with six); 300 rows of three parts take 7.3 us with four and 8.6 with six.
+    auto kernel = u == 4 ? add_rmsnorm_fp8_kernel<A, W, 4, 1> : u == 2 ? (p.parts > 1 ? add_rmsnorm_fp8_kernel<A, W, 2, 2> : add_rmsnorm_fp8_kernel<A, W, 2, 1>)
+                : p.parts == 1 ? add_rmsnorm_fp8_kernel<A, W, 1, 1> : threads <= 640 && n <= multiprocessors() ? add_rmsnorm_fp8_kernel<A, W, 1, ALONE> : add_rmsnorm_fp8_kernel<A, W, 1, 4>;
+    launch_overlapped(kernel, dim3(n), dim3(threads), 0, stream, p);
     return check_launch("add_rmsnorm_fp8");
 }
 

@@ -121,7 +121,7 @@ def test_rows_past_two_to_the_31():
 
 
 @pytest.mark.parametrize("E", [1, 64, 127, 128, 1000, 1002, 2056, 4096, 5120, 8200, 16400, 32768])
-@pytest.mark.parametrize("add,parts", [(None, 1), ("f32", 1), ("bf16", 1), ("f32", 3)])
+@pytest.mark.parametrize("add,parts", [(None, 1), ("f32", 1), ("bf16", 1), ("f32", 3), ("f32", 9), ("bf16", 7)])
 def test_add_rmsnorm(E, add, parts):
     from purhie_b200.csrc import fp8
     T, eps = 5, 1e-5
@@ -142,6 +142,24 @@ def test_add_rmsnorm(E, add, parts):
     v = out.double()
     y = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps) * w.double()
     check_quantized(q, s, y, 1, 100 * U)
+
+
+@pytest.mark.parametrize("E", [1000, 5120, 5248, 8320])
+@pytest.mark.parametrize("parts", [2, 5, 9, 13])
+def test_a_row_s_norm_does_not_depend_on_the_others(parts, E):
+    """More rows than multiprocessors and few: the same bits."""
+    from purhie_b200.csrc import fp8
+    T = 2 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+    x, a, w = rnd(T, E, seed=E), rnd(parts, T, E, seed=parts), 1 + 0.3 * rnd(E, seed=2)
+    out = torch.empty_like(x)
+    q, s = fp8.add_rmsnorm(x, a, w, 1e-6, add_splits=parts, x_out=out)
+    v = x.clone()
+    for i in range(parts):
+        v += a[i]
+    assert torch.equal(out, v)
+    few = torch.empty(3, E, device=DEV)
+    q1, s1 = fp8.add_rmsnorm(x[7:10].contiguous(), a[:, 7:10].contiguous(), w, 1e-6, add_splits=parts, x_out=few)
+    assert torch.equal(few, out[7:10]) and torch.equal(q1.view(torch.uint8), q[7:10].view(torch.uint8)) and torch.equal(s1, s[7:10])
 
 
 def test_add_rmsnorm_keeps_the_sum_where_told():
@@ -177,7 +195,7 @@ def gate_value(g, u, gate):
 
 
 @pytest.mark.parametrize("gate", [None, (1.702, 7.0, 1.0), "gelu_tanh"])
-@pytest.mark.parametrize("dtype,parts", [("f32", 1), ("bf16", 1), ("f32", 3)])
+@pytest.mark.parametrize("dtype,parts", [("f32", 1), ("bf16", 1), ("f32", 3), ("f32", 7), ("bf16", 4)])
 @pytest.mark.parametrize("T,F", [(1, 1), (3, 127), (2, 128), (5, 1000), (4, 1001), (7, 1002), (33, 4104)])
 def test_gated(T, F, dtype, parts, gate):
     from purhie_b200.csrc import fp8
