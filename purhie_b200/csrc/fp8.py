@@ -179,7 +179,11 @@ def _gate(gate):
         return None
     if isinstance(gate, str) and gate != "gelu_tanh":
         raise KernelError(f"gated: gate {gate!r} is not known")
-    return (c_float * 4)(0, 0, 0, 2) if isinstance(gate, str) else (c_float * 4)(*gate, 1)
+    if isinstance(gate, str):
+        return (c_float * 4)(0, 0, 0, 2)
+    if len(gate) != 3:
+        raise KernelError(f"gated: the clamped swish has alpha, limit and shift, got {tuple(gate)}")
+    return (c_float * 4)(*gate, 1)
 
 
 def gated(gate_up: torch.Tensor, out: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None, *, splits: int = 1,

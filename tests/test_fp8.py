@@ -47,6 +47,8 @@ REFUSED = [
     ("gate_up", lambda: fp8.gated(f32(2, 128)[:, :64])),
     ("CUDA", lambda: fp8.gated(f32(2, 64))),
     ("gate 'relu'", lambda: fp8._gate("relu")),
+    ("alpha, limit and shift", lambda: fp8._gate((1.702, 7.0))),
+    ("alpha, limit and shift", lambda: fp8._gate((1.702, 7.0, 1.0, 0.0))),
     ("float8", lambda: fp8.gemm(bf16(2, 64), f32(2, 1), e4m3(8, 64), f32(1, 1))),
     ("float8", lambda: fp8.gemm(e4m3(64, 2).t(), f32(2, 1), e4m3(8, 64), f32(1, 1))),
     ("do not fit", lambda: fp8.gemm(e4m3(2, 64), f32(2, 1), e4m3(8, 32), f32(1, 1))),
