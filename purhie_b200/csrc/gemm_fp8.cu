@@ -817,7 +817,9 @@ int launch(const void* x, const void* w, Params p, int K, cudaStream_t stream) {
 // times (an item's start and end + its blocks of K), the weight's way from memory and the tiles' from L2, and for several parts
 // their way out and back and the kernel that adds them up, or what they cost whoever consumes them.  Fitted to 1,538 launches at 1 to 2,048
 // tokens, 256 to 24,576 features and K 512 to 16,384 (root mean square error 5 %); what it picks takes 1.5 % longer than the
-// best of all, over those 80 products.  (Tiles of 128 tokens were never the best by more than 1 %, and are gone.)
+// best of all, over those 80 products.  (Tiles of 128 tokens, with four epilogue warps, were never the best by more than 1 %; with eight and an
+// SM for each CTA 128 x 24576 x 4096 took 40 us for 43, 256 rows 64 for 44: a product of 128 x 128 takes from shared memory, and the
+// copies bring into it, what that moves in a block's time.  They are gone.)
 // Parts that are handed on cost their consumer 0.8 us and 0.1 us each: with that, one row through the products, norms and
 // quantizers of a layer of the 8B shape takes 46.5 us and not 48.3 (gate and up whole, not in three parts).
 void choose(int M, int N, int K, int sms, bool whole, int* tile, int* splits) {
