@@ -468,6 +468,41 @@ def test_feed_forward_in_graphs_and_streams():
     fp8.check_errors()
 
 
+def test_many_rows_in_graphs_and_streams():
+    """The same for rows enough for pairs of CTAs, the activation in the first product's epilogue."""
+    from purhie_b200.csrc import fp8
+    E, F, T = 416, 1024, 700
+    norm, up, up_s, down, down_s = weights(E, F)
+
+    def run(x, add):
+        q, s = fp8.add_rmsnorm(x, add, norm, 1e-6, x_out=torch.empty_like(x))
+        q2, s2 = fp8.gemm_gated(q, s, up, up_s)
+        return fp8.gemm(q2, s2, down, down_s, out_dtype=torch.float32, tile=256)
+    inputs = [(rnd(T, E, seed=10 + i), rnd(T, E, seed=20 + i).to(torch.bfloat16)) for i in range(4)]
+    want = [run(*i).clone() for i in inputs]
+    held = [(torch.zeros(T, E, device=DEV), torch.zeros(T, E, device=DEV).to(torch.bfloat16)) for _ in range(2)]
+    graphs = []
+    for h in held:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run(*h)
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(0, 4, 2):
+        for j in range(2):
+            held[j][0].copy_(inputs[i + j][0])
+            held[j][1].copy_(inputs[i + j][1])
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for j in range(2):
+                with torch.cuda.stream(streams[j]):
+                    graphs[j][0].replay()
+        torch.cuda.synchronize()
+        for j in range(2):
+            assert torch.equal(graphs[j][1], want[i + j])
+    fp8.check_errors()
+
+
 def test_plain_calls_and_checked_ones_are_the_same():
     """A call without outputs takes the compiled step, one with them the checks of the face: the same launches."""
     from purhie_b200.csrc import fp8, ops
