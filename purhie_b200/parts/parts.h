@@ -57,14 +57,15 @@ inline const char* role_name(Role r) { return r == Role::Matrix ? "matrix" : r =
 // Where a part gets its tensors from while it binds: a checkpoint folder or the random generator.  fetch()
 // returns the tensor on the device in the dtype the policy gives it (matrix: the compute dtype, except that a
 // tensor stored in 32-bit stays 32-bit; vector: float32; table: int32).  The part owns what it keeps: tensors
-// from fetch() stay alive as long as the model's arena; release() gives a temporary back early.
+// from fetch() stay alive as long as the model's arena; release() gives a temporary back early (a tensor that was fetched more than
+// once stays: another part may keep it).
 class QE_API WeightSource {
 public:
     virtual ~WeightSource() = default;
     virtual Tensor fetch(const std::string& name) = 0;
     virtual DeviceArena& arena() = 0;
     virtual cudaStream_t stream() = 0;
-    void release(const Tensor& t) { arena().release(t); }
+    virtual void release(const Tensor& t) { arena().release(t); }
 };
 
 // ---- what the cache manager keeps for one run-order entry ----------------------------------------------------

@@ -63,6 +63,22 @@ FolderSource::FolderSource(const std::string& model_dir, const std::vector<Tenso
 }
 
 namespace {
+// Gives t back to the arena, and forgets it, unless it was handed out more than once.
+void release_fetched(FetchedTensors& fetched, DeviceArena& arena, const Tensor& t) {
+    for (auto it = fetched.begin(); it != fetched.end(); ++it) {
+        if (it->second.tensor.data != t.data) continue;
+        if (it->second.times > 1) return;
+        fetched.erase(it);
+        break;
+    }
+    arena.release(t);
+}
+}  // namespace
+
+void FolderSource::release(const Tensor& t) { release_fetched(cache_, arena_, t); }
+void RandomSource::release(const Tensor& t) { release_fetched(cache_, arena_, t); }
+
+namespace {
 double read_as_double(const uint8_t* p, DType d, size_t i) {
     switch (d) {
         case DType::F64: { double v; memcpy(&v, p + 8 * i, 8); return v; }
@@ -80,7 +96,7 @@ double read_as_double(const uint8_t* p, DType d, size_t i) {
 
 Tensor FolderSource::fetch(const std::string& name) {
     auto hit = cache_.find(name);
-    if (hit != cache_.end()) return hit->second;
+    if (hit != cache_.end()) { hit->second.times++; return hit->second.tensor; }
     auto sp = specs_.find(name);
     if (sp == specs_.end()) throw Error(kInvalidState, "a part asks for the tensor '" + name + "' that it did not announce");
     const TensorEntry& e = folder_.at(name);
@@ -110,7 +126,7 @@ Tensor FolderSource::fetch(const std::string& name) {
         // does not wait for the default stream, must find all of it.
         QE_CUDA(cudaStreamSynchronize(nullptr));
     }
-    cache_[name] = t;
+    cache_[name] = {t, 1};
     return t;
 }
 
@@ -133,7 +149,7 @@ RandomSource::RandomSource(const std::vector<TensorSpec>& expected, const Random
 
 Tensor RandomSource::fetch(const std::string& name) {
     auto hit = cache_.find(name);
-    if (hit != cache_.end()) return hit->second;
+    if (hit != cache_.end()) { hit->second.times++; return hit->second.tensor; }
     auto sp = specs_.find(name);
     if (sp == specs_.end()) throw Error(kInvalidState, "a part asks for the tensor '" + name + "' that it did not announce");
     const TensorSpec& spec = sp->second;
@@ -156,7 +172,7 @@ Tensor RandomSource::fetch(const std::string& name) {
     } else {
         QE_LAUNCH(k, k.random_fill(t.data, t.code(), t.numel(), key, kind, a, b, stream_));
     }
-    cache_[name] = t;
+    cache_[name] = {t, 1};
     return t;
 }
 

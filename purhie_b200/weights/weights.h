@@ -40,6 +40,13 @@ QE_API void check_folder(const SafetensorsFolder& folder, const std::vector<Tens
                          const std::vector<std::string>& ignore);
 
 // Tensors from a checkpoint folder (checked against `expected` when constructed).
+// What a source has handed out under a name, and how often.
+struct FetchedTensor {
+    Tensor tensor;
+    int times = 0;
+};
+using FetchedTensors = std::map<std::string, FetchedTensor>;
+
 class QE_API FolderSource : public WeightSource {
 public:
     FolderSource(const std::string& model_dir, const std::vector<TensorSpec>& expected, const std::vector<std::string>& ignore,
@@ -47,10 +54,11 @@ public:
     Tensor fetch(const std::string& name) override;
     DeviceArena& arena() override { return arena_; }
     cudaStream_t stream() override { return stream_; }
+    void release(const Tensor& t) override;
 private:
     SafetensorsFolder folder_;
     std::map<std::string, TensorSpec> specs_;
-    std::map<std::string, Tensor> cache_;
+    FetchedTensors cache_;
     DType compute_;
     DeviceArena& arena_;
     cudaStream_t stream_;
@@ -65,9 +73,10 @@ public:
     Tensor fetch(const std::string& name) override;
     DeviceArena& arena() override { return arena_; }
     cudaStream_t stream() override { return stream_; }
+    void release(const Tensor& t) override;
 private:
     std::map<std::string, TensorSpec> specs_;
-    std::map<std::string, Tensor> cache_;
+    FetchedTensors cache_;
     RandomInit init_;
     DType stored_, compute_;
     DeviceArena& arena_;

@@ -204,6 +204,25 @@ def test_weights_are_whole_before_they_are_brought_to_8_bits(tmp_path):
         assert np.linalg.norm((g - want)[:, 256:]) < 0.1 * np.linalg.norm(want[:, 256:])
 
 
+@pytest.mark.parametrize("options", [{"gemm": "fp8"}, {"gemm": "auto"}])
+def test_a_matrix_under_one_name_for_two_products(options, tmp_path):
+    """What the first product does with the weight when it is bound leaves the second one its own."""
+    from purhie_b200.csrc.build import build_library
+    from purhie_b200.parts import PartProbe
+    build_library("fp8")
+    E = 272
+    w = (torch.randn(E, E, generator=torch.Generator().manual_seed(5)) * E ** -0.5).to(torch.bfloat16)
+    got = []
+    for i, names in enumerate(({"up_proj": "w", "down_proj": "w"}, {"up_proj": "w", "down_proj": "v"})):
+        d = tmp_path / str(i)
+        d.mkdir()
+        save_file({n: w.clone() for n in set(names.values())}, str(d / "model.safetensors"))
+        probe = PartProbe("feed_forward", "mlp", {"hidden_size": E, "intermediate_size": E, "activation": "silu", "names": names}, "bfloat16", options)
+        probe.bind_folder(str(d))
+        got.append(probe.feed_forward(torch.randn(9, E, generator=torch.Generator().manual_seed(6)).numpy()))
+    assert np.isfinite(got[0]).all() and np.abs(got[0]).max() > 0 and np.array_equal(got[0], got[1])
+
+
 def test_matrices_that_do_not_fit_stay_as_they_are(tmp_path):
     """Rows of a number of values that is no multiple of 16 stay in bfloat16: the same bits as without the option."""
     E, F = 264, 656
