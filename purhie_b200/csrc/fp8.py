@@ -232,7 +232,7 @@ def gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: tor
     [ceil(N / 128), ceil(K / 128)], K a multiple of 16, sums in float32, out float32 or bfloat16 (``out_dtype`` where out is not
     given).  ``splits`` > 1: K is cut into that many parts and out is [splits, M, N] float32, the sums of each, for a consumer that
     adds them up (``add_rmsnorm``, ``gated``); 0: cut as the kernel likes it, and out is the whole sum.  ``tile`` (0: the kernel's own
-    choice): 16, 32 or 64 tokens beside 128 features, or 256 x 256 on pairs of CTAs.  ``early_w``: w is not the result of a
+    choice): 16, 32, 64 or 96 tokens beside 128 features, or 256 x 256 on pairs of CTAs.  ``early_w``: w is not the result of a
     kernel that may still run when the product starts (a model's weight), so its first tiles may be read before the kernel in
     front has ended."""
     if out is None and not tile and not splits and (out_dtype is torch.bfloat16 or out_dtype is F32):

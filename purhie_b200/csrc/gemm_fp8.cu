@@ -151,12 +151,12 @@ template <int BN> struct Tile {
     static constexpr int STAGE_BYTES = A_BYTES + BN * BK;
     static constexpr int CTAS_PER_SM = 2;
     static constexpr int STAGES = 96 * 1024 / STAGE_BYTES;
-    static constexpr int BUFFERS = BN == 64 ? 4 : 128 / BN;              // accumulators in tensor memory
-    static constexpr int TMEM_COLS = BUFFERS * BN;
+    static constexpr int TMEM_COLS = BN >= 64 ? 256 : 128;
+    static constexpr int BUFFERS = TMEM_COLS / BN;                       // accumulators in tensor memory
     static constexpr int FACTORS_LD = BN + 4;                            // (lanes write down a column: on eight banks, not on one)
     static constexpr int FACTORS_BYTES = FACTOR_BLOCKS * FACTORS_LD * 4;
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + FACTORS_BYTES + 256;
-    static constexpr int CHUNK = BN == 64 ? 32 : 16;                     // columns of an accumulator that are read at a time
+    static constexpr int CHUNK = BN >= 64 ? 32 : 16;                     // columns of an accumulator that are read at a time
     static_assert(TMEM_COLS * CTAS_PER_SM <= 512, "tensor memory");
     static_assert((2 * STAGES + 2 * BUFFERS) * 8 + 4 <= 256, "barriers");
 };
@@ -812,19 +812,19 @@ int launch(const void* x, const void* w, Params p, int K, cudaStream_t stream) {
     return check_launch("gemm_fp8");
 }
 
-// The tile (16, 32 or 64 tokens beside 128 features; 256: pairs) and the parts of K with the least estimated time, among those that
+// The tile (16, 32, 64 or 96 tokens beside 128 features; 256: pairs) and the parts of K with the least estimated time, among those that
 // the caller leaves open (0).  Microseconds: a launch (a pair's does not start early), rounds of the CTAs over the device's places
 // times (an item's start and end + its blocks of K), the weight's way from memory and the tiles' from L2, and for several parts
 // their way out and back and the kernel that adds them up, or what they cost whoever consumes them.  Fitted to 1,538 launches at 1 to 2,048
 // tokens, 256 to 24,576 features and K 512 to 16,384 (root mean square error 5 %); what it picks takes 1.5 % longer than the
-// best of all, over those 80 products.  (Tiles of 128 tokens, with four epilogue warps, were never the best by more than 1 %; with eight and an
-// SM for each CTA 128 x 24576 x 4096 took 40 us for 43, 256 rows 64 for 44: a product of 128 x 128 takes from shared memory, and the
-// copies bring into it, what that moves in a block's time.  They are gone.)
+// best of all, over those 80 products.  Tiles of 96 tokens, fitted to 327 more, are for 65 to 96 rows of wide weights: 72 x 24576 x 4096 takes
+// 29 us in one, 38 in three of 32.  (Tiles of 128 tokens, with four epilogue warps, were never the best by more than 1 %; with eight and an
+// SM for each CTA 128 x 24576 x 4096 took 40 us for 43, but 256 rows 64 for 44.  They are gone.)
 // Parts that are handed on cost their consumer 0.8 us and 0.1 us each: with that, one row through the products, norms and
 // quantizers of a layer of the 8B shape takes 46.5 us and not 48.3 (gate and up whole, not in three parts).
 void choose(int M, int N, int K, int sms, bool whole, int* tile, int* splits) {
     struct Kind { int tile, per_sm; double launch, item, block; };
-    static const Kind kinds[] = {{16, 2, 0.26, 1.92, 0.339}, {32, 2, 0.26, 2.34, 0.358}, {64, 2, 0.26, 3.61, 0.404}, {256, 0, 4.08, 1.54, 0.491}};
+    static const Kind kinds[] = {{16, 2, 0.26, 1.92, 0.339}, {32, 2, 0.26, 2.34, 0.358}, {64, 2, 0.26, 3.61, 0.404}, {96, 2, 0.26, 4.84, 0.54}, {256, 0, 4.08, 1.54, 0.491}};
     const int kblocks = (K + BK - 1) / BK, asked_tile = *tile, asked_splits = *splits;
     const double weight_mb = 1e-6 * N * K;
     double best = -1.0;
@@ -850,13 +850,13 @@ void choose(int M, int N, int K, int sms, bool whole, int* tile, int* splits) {
 PH_EXPORT int ph_gemm_fp8_plan(int M, int N, int K, int whole, int* tile, int* splits) {
     if (M < 1 || N < 1 || K < 1 || M > MAX_SIZE || N > MAX_SIZE || K > MAX_SIZE || !tile || !splits || *tile < 0 || *splits < 0) return fail(PH_ERR_ARG, "gemm_fp8: no plan for M %d, N %d, K %d", M, N, K);
     const int kblocks = (K + BK - 1) / BK;
-    if (*tile != 0 && *tile != 16 && *tile != 32 && *tile != 64 && *tile != 256) return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 256", *tile);
+    if (*tile != 0 && *tile != 16 && *tile != 32 && *tile != 64 && *tile != 96 && *tile != 256) return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 96, 256", *tile);
     if (*splits > kblocks || *splits > MAX_SPLITS) return fail(PH_ERR_ARG, "gemm_fp8: %d parts of K for %d blocks (at most %d)", *splits, kblocks, MAX_SPLITS);
     choose(M, N, K, multiprocessors(), whole != 0, tile, splits);
     return PH_OK;
 }
 
-// out = x times w transposed, with scales (above); xs [M, ceil(K / 128)], ws [ceil(N / 128), ceil(K / 128)].  tile: 16, 32 or 64 tokens
+// out = x times w transposed, with scales (above); xs [M, ceil(K / 128)], ws [ceil(N / 128), ceil(K / 128)].  tile: 16, 32, 64 or 96 tokens
 // beside 128 features, or 256: 256 x 256 on pairs of CTAs.  splits: parts of K, 1 to 16.  With several, parts is room for
 // [splits][M, N] float32: the sums of each part go there, and then, where out is given, their sum to out.  With one, or for the sum,
 // out [M, N] is float32 or bfloat16.  early_w: w and ws are not results of a kernel that may still run when this one starts, and the first
@@ -881,10 +881,11 @@ PH_EXPORT int ph_gemm_fp8(const void* x, const float* xs, const void* w, const f
         case 16: rc = launch<16>(x, w, p, K, stream); break;
         case 32: rc = launch<32>(x, w, p, K, stream); break;
         case 64: rc = launch<64>(x, w, p, K, stream); break;
+        case 96: rc = launch<96>(x, w, p, K, stream); break;
         case 256:
             rc = launch_pair(x, w, p, K, stream);
             break;
-        default: return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 256", tile);
+        default: return fail(PH_ERR_ARG, "gemm_fp8: tile %d is not one of 16, 32, 64, 96, 256", tile);
     }
     if (rc != PH_OK || splits == 1 || !out) return rc;
     const long long values = (long long)M * N, grid = (values + 1023) / 1024;

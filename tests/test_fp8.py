@@ -115,7 +115,7 @@ def test_launchers_refuse(text, name, args):
 def test_plans(M, N, K, whole):
     """What a plan gives can be launched, and what the caller gave stays."""
     tile, splits = fp8.plan(M, N, K, whole=whole)
-    assert tile in (16, 32, 64, 256) and 1 <= splits <= min(16, -(-K // 128))
+    assert tile in (16, 32, 64, 96, 256) and 1 <= splits <= min(16, -(-K // 128))
     for given in (16, 256):
         assert fp8.plan(M, N, K, tile=given)[0] == given
     assert fp8.plan(M, N, K, splits=1)[1] == 1

@@ -271,7 +271,7 @@ SHAPES = [(1, 16), (64, 128), (100, 48), (129, 144), (257, 272), (1000, 2064), (
 
 @pytest.mark.parametrize("out", ["f32", "bf16"])
 @pytest.mark.parametrize("N,K", SHAPES)
-@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 32, 33, 64, 65, 128, 129, 300])
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 32, 33, 64, 65, 96, 97, 128, 129, 300])
 def test_product(M, N, K, out):
     from purhie_b200.csrc import fp8
     x, xs, w, ws = operands(M, N, K, M + N + K)
@@ -280,7 +280,7 @@ def test_product(M, N, K, out):
     fp8.check_errors()
 
 
-@pytest.mark.parametrize("tile,splits", [(t, s) for t in (16, 32, 64, 256) for s in (1, 2, 3, 7, 16)])
+@pytest.mark.parametrize("tile,splits", [(t, s) for t in (16, 32, 64, 96, 256) for s in (1, 2, 3, 7, 16)])
 @pytest.mark.parametrize("M,N", [(1, 200), (40, 200), (150, 200), (290, 515)])
 def test_product_of_every_tile_and_split(M, N, splits, tile):
     """Small whole numbers and scales that are powers of two: every sum is exact in float32, so every variant gives the same bits."""
@@ -308,7 +308,7 @@ def test_product_of_every_tile_and_split(M, N, splits, tile):
 def test_product_into_places_off_their_boundaries():
     """Outputs that start on their own type's boundary only, at widths whose rows would allow vectors."""
     from purhie_b200.csrc import fp8
-    for M, N, K, tile in ((3, 260, 1040, 16), (70, 132, 2064, 64), (300, 264, 400, 256)):
+    for M, N, K, tile in ((3, 260, 1040, 16), (70, 132, 2064, 64), (90, 132, 2064, 96), (300, 264, 400, 256)):
         x, xs, w, ws = operands(M, N, K, M)
         for dtype in DT.values():
             held = torch.zeros(M * N + 9, dtype=dtype, device=DEV)
