@@ -59,7 +59,8 @@ def _stream(what: str, first: torch.Tensor, *others) -> int:
             raise KernelError(f"{what}: the tensors are not all on one device")
     if at != torch.cuda.current_device():
         raise KernelError(f"{what}: the tensors are on device {at}, which is not the current one")
-    return ops._stream_now if ops._stream_now is not None else _raw_stream(at)
+    scope = ops._scope.stream
+    return scope if scope is not None else _raw_stream(at)
 
 
 _calls = None
@@ -76,7 +77,8 @@ def _load_calls():
 
 
 def _scope() -> int:
-    return -1 if ops._stream_now is None else ops._stream_now
+    scope = ops._scope.stream
+    return -1 if scope is None else scope
 
 
 def _made(got):

@@ -9,6 +9,7 @@ implementation: a missing library is an error.
 from __future__ import annotations
 
 import ctypes
+import threading
 from ctypes import c_double, c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
@@ -56,27 +57,30 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-_stream_now: Optional[int] = None
+class _Scope(threading.local):
+    """The stream of the on_current_stream() scope that this thread is in."""
+    stream: Optional[int] = None
+
+
+_scope = _Scope()
 
 
 def _stream() -> int:
     """The stream the launchers use: the current one, looked up once per :func:`on_current_stream` scope."""
-    return _stream_now if _stream_now is not None else torch.cuda.current_stream().cuda_stream
+    return _scope.stream if _scope.stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 class on_current_stream:
-    """Inside this scope every launcher uses the stream that was current when the scope was entered, without asking
-    torch again for each of the few hundred launches of a step."""
+    """Inside this scope every launcher that the thread calls uses the stream that was current when the scope was entered,
+    without asking torch again for each of the few hundred launches of a step."""
 
     def __enter__(self):
-        global _stream_now
-        self._before = _stream_now
-        _stream_now = torch.cuda.current_stream().cuda_stream
+        self._before = _scope.stream
+        _scope.stream = torch.cuda.current_stream().cuda_stream
         return self
 
     def __exit__(self, *exc):
-        global _stream_now
-        _stream_now = self._before
+        _scope.stream = self._before
         return False
 
 
