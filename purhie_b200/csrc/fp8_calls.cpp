@@ -6,6 +6,7 @@
 //
 // The kernels' launchers are handed over by address (set_launchers): this file links against torch and nothing else here does.
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -37,7 +38,18 @@ int code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.sca
 bool fits(const at::Tensor& t, at::ScalarType type, int device) { return t.is_cuda() && t.get_device() == device && t.scalar_type() == type && t.is_contiguous(); }
 bool is(const at::Tensor& t, int64_t a, int64_t b) { return t.dim() == 2 && t.size(0) == a && t.size(1) == b; }
 bool size_ok(int64_t n) { return n > 0 && n <= MOST; }
-cudaStream_t stream_of(int device, int64_t given) { return given >= 0 ? (cudaStream_t)given : c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
+// The stream that a launch goes to: the scope's (`given`, where it is not negative), else the current one.  While this lives it is the
+// current one, so that new tensors are of its memory: another stream's would be handed out again there while the launch still
+// works on it.
+struct LaunchStream {
+    cudaStream_t stream;
+    c10::cuda::OptionalCUDAStreamGuard guard;
+    LaunchStream(int device, int64_t given) : stream(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream()) {
+        if (given < 0 || (cudaStream_t)given == stream) return;
+        stream = (cudaStream_t)given;
+        guard.reset_stream(c10::cuda::getStreamFromExternal(stream, (c10::DeviceIndex)device));
+    }
+};
 at::Tensor matrix(int64_t rows, int64_t columns, const at::Tensor& like, at::ScalarType type) { return at::empty({rows, columns}, like.options().dtype(type)); }
 
 // What a launch gave: its outputs, or the status that the face turns into the library's error.
@@ -52,8 +64,9 @@ py::object quantize(const at::Tensor& x, int64_t block_rows, int64_t given) {
     const int64_t T = x.size(0), K = x.size(1), apart = x.stride(0);
     const int device = x.get_device(), type = code(x);
     if (device != c10::cuda::current_device() || type < 0 || !size_ok(T) || !size_ok(K) || (x.stride(1) != 1 && K > 1) || (T > 1 && apart < K)) return py::none();
+    LaunchStream launch(device, given);
     at::Tensor q = matrix(T, K, x, E4M3), scales = matrix(block_rows == 1 ? T : blocks(T), blocks(K), x, at::kFloat);
-    return outcome(g_quantize(x.data_ptr(), type, T > 1 ? apart : K, q.data_ptr(), (float*)scales.data_ptr(), (int)T, (int)K, (int)block_rows, stream_of(device, given)), q, scales);
+    return outcome(g_quantize(x.data_ptr(), type, T > 1 ? apart : K, q.data_ptr(), (float*)scales.data_ptr(), (int)T, (int)K, (int)block_rows, launch.stream), q, scales);
 }
 
 py::object add_rmsnorm(const at::Tensor& x, const std::optional<at::Tensor>& add, const at::Tensor& weight, double eps, int64_t parts, bool write_x,
@@ -77,9 +90,10 @@ py::object add_rmsnorm(const at::Tensor& x, const std::optional<at::Tensor>& add
     } else if (write_x && add) {
         keep = x.data_ptr();
     }
+    LaunchStream launch(device, given);
     at::Tensor q = matrix(T, E, x, E4M3), scales = matrix(T, blocks(E), x, at::kFloat);
     return outcome(g_norm((const float*)x.data_ptr(), add ? add->data_ptr() : nullptr, type, (int)parts, T * E, (const float*)weight.data_ptr(), (float)eps, nullptr, (int)T, (int)T,
-                          (int)E, (float*)keep, q.data_ptr(), (float*)scales.data_ptr(), stream_of(device, given)), q, scales);
+                          (int)E, (float*)keep, q.data_ptr(), (float*)scales.data_ptr(), launch.stream), q, scales);
 }
 
 py::object gated(const at::Tensor& gate_up, int64_t parts, int64_t given) {
@@ -88,8 +102,9 @@ py::object gated(const at::Tensor& gate_up, int64_t parts, int64_t given) {
     const int64_t T = gate_up.size(-2), width = gate_up.size(-1), F = width / 2;
     const int device = gate_up.get_device(), type = code(gate_up);
     if (device != c10::cuda::current_device() || type < 0 || !size_ok(T) || !size_ok(width) || width % 2 || !gate_up.is_contiguous()) return py::none();
+    LaunchStream launch(device, given);
     at::Tensor q = matrix(T, F, gate_up, E4M3), scales = matrix(T, blocks(F), gate_up, at::kFloat);
-    return outcome(g_gated(gate_up.data_ptr(), type, (int)parts, T * width, q.data_ptr(), (float*)scales.data_ptr(), (int)T, (int)F, nullptr, stream_of(device, given)), q, scales);
+    return outcome(g_gated(gate_up.data_ptr(), type, (int)parts, T * width, q.data_ptr(), (float*)scales.data_ptr(), (int)T, (int)F, nullptr, launch.stream), q, scales);
 }
 
 // The whole product, cut as the plan says; bf16: of the output.
@@ -102,10 +117,11 @@ py::object gemm(const at::Tensor& x, const at::Tensor& xs, const at::Tensor& w, 
         return py::none();
     int tile = 0, splits = 0;
     if (const int status = g_plan((int)M, (int)N, (int)K, 1, &tile, &splits)) return py::int_(status);
+    LaunchStream launch(device, given);
     at::Tensor out = matrix(M, N, x, bf16 ? at::kBFloat16 : at::kFloat), parts;
     if (splits > 1) parts = at::empty({splits, M, N}, x.options().dtype(at::kFloat));
     const int status = g_gemm(x.data_ptr(), (const float*)xs.data_ptr(), w.data_ptr(), (const float*)ws.data_ptr(), out.data_ptr(), bf16 ? 1 : 0, (int)M, (int)N, (int)K, tile, splits,
-                              splits > 1 ? (float*)parts.data_ptr() : nullptr, early_w ? 1 : 0, nullptr, stream_of(device, given));
+                              splits > 1 ? (float*)parts.data_ptr() : nullptr, early_w ? 1 : 0, nullptr, launch.stream);
     if (status != 0) return py::int_(status);
     return py::cast(out);
 }

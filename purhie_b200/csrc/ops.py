@@ -40,7 +40,7 @@ class Workspace:
         if buf is None or buf.numel() < n:
             if self.frozen:
                 raise RuntimeError(f"workspace buffer {name!r} would have to grow while frozen")
-            buf = torch.empty(max(n, 1), dtype=dtype, device=self.device)
+            buf = of_launch_stream(torch.empty, max(n, 1), dtype=dtype, device=self.device)
             self._bufs[(name, dtype)] = buf
         return buf[:n].view(*shape)
 
@@ -58,8 +58,9 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 class _Scope(threading.local):
-    """The stream of the on_current_stream() scope that this thread is in."""
+    """The stream of the on_current_stream() scope that this thread is in: its handle, and the stream itself."""
     stream: Optional[int] = None
+    whole: Optional[torch.cuda.Stream] = None
 
 
 _scope = _Scope()
@@ -75,13 +76,24 @@ class on_current_stream:
     without asking torch again for each of the few hundred launches of a step."""
 
     def __enter__(self):
-        self._before = _scope.stream
-        _scope.stream = torch.cuda.current_stream().cuda_stream
+        self._before = _scope.stream, _scope.whole
+        _scope.whole = torch.cuda.current_stream()
+        _scope.stream = _scope.whole.cuda_stream
         return self
 
     def __exit__(self, *exc):
-        _scope.stream = self._before
+        _scope.stream, _scope.whole = self._before
         return False
+
+
+def of_launch_stream(make, *args, **kwargs) -> torch.Tensor:
+    """A new tensor, make(...), from the memory of the stream that the launchers use.  Inside a scope another stream may be the
+    current one; memory of that one would be its own to hand out again as soon as the tensor is dropped, while the launch on
+    the scope's stream still works on it."""
+    if _scope.stream is None or _scope.stream == torch._C._cuda_getCurrentRawStream(_scope.whole.device_index):
+        return make(*args, **kwargs)
+    with torch.cuda.stream(_scope.whole):
+        return make(*args, **kwargs)
 
 
 def _need(t: torch.Tensor, name: str, dtype=None) -> torch.Tensor:
@@ -204,7 +216,7 @@ def add_weight_sumsq(x: torch.Tensor, add: Optional[torch.Tensor], weight: torch
     E = x.shape[-1]
     T = x.numel() // E
     chunks = -(-E // 512)
-    sumsq = torch.empty(T, chunks, dtype=torch.float32, device=x.device)
+    sumsq = of_launch_stream(torch.empty, T, chunks, dtype=torch.float32, device=x.device)
     if add is not None:
         _need(add, "add")
         if add.numel() != add_splits * T * E:
@@ -412,8 +424,8 @@ def attention_talking_mma(q, k_base, v_base, page_stride, page_size, block_table
     """The tensor-core kernel (bfloat16): tiles of 16 rows of one request, all heads per tile."""
     _need(q, "q", torch.bfloat16); _need(out, "out", torch.bfloat16)
     T = q.shape[0]
-    part_o = torch.empty((T, num_heads, splits, head_dim), dtype=torch.float32, device=q.device) if splits > 1 else None
-    part_ml = torch.empty((T, num_heads, splits, 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+    part_o = of_launch_stream(torch.empty, (T, num_heads, splits, head_dim), dtype=torch.float32, device=q.device) if splits > 1 else None
+    part_ml = of_launch_stream(torch.empty, (T, num_heads, splits, 2), dtype=torch.float32, device=q.device) if splits > 1 else None
     call("core", "ph_attention_talking_mma", _ptr(q), _ptr(k_base), _ptr(v_base), page_stride, page_size, _ptr(block_table),
          block_table.shape[-1], _ptr(seg_start), _ptr(seg_ctx), _ptr(tile_seg), _ptr(tile_first), tile_seg.numel(), _ptr(out), num_heads,
          num_kv_heads, head_dim, head_dim, int(window or 0), 0, float(scale), float(cap), _ptr(slope), _ptr(rate), _ptr(talk), _ptr(sink),
@@ -427,7 +439,7 @@ def min_gru_scan(rows: torch.Tensor, z_bias, x_bias, state, seg_start, seg_slot,
     splits, T, width3 = rows.shape
     W = width3 // 3
     n_chunks = 0 if chunks is None else chunks.numel() // 4
-    carry = torch.empty((3, max(n_chunks, 1), W), dtype=torch.float32, device=rows.device)
+    carry = of_launch_stream(torch.empty, (3, max(n_chunks, 1), W), dtype=torch.float32, device=rows.device)
     call("core", "ph_min_gru_scan", _ptr(rows), _code(rows.dtype), splits, T * width3, width3, _ptr(z_bias), _ptr(x_bias), _ptr(state),
          _ptr(seg_start), _ptr(seg_slot), seg_slot.numel(), T, W, _ptr(chunks), n_chunks, _ptr(seg_chunks), _ptr(carry), _ptr(out),
          _code(out.dtype), _stream())
