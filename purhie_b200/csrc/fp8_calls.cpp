@@ -58,15 +58,24 @@ py::object outcome(int status, const at::Tensor& a, const at::Tensor& b) {
     return py::make_tuple(a, b);
 }
 
-// given: the stream of a scope that has one (>= 0), else -1.
+// given: the stream of a scope that has one (>= 0), else -1.  Tensors are made and kernels launched without the interpreter's lock, as
+// through ctypes and torch: either waits where memory or the device's queue is full, and what it waits for may need another
+// thread of Python.
 py::object quantize(const at::Tensor& x, int64_t block_rows, int64_t given) {
     if (!x.is_cuda() || x.dim() != 2 || (block_rows != 1 && block_rows != BLOCK)) return py::none();
     const int64_t T = x.size(0), K = x.size(1), apart = x.stride(0);
     const int device = x.get_device(), type = code(x);
     if (device != c10::cuda::current_device() || type < 0 || !size_ok(T) || !size_ok(K) || (x.stride(1) != 1 && K > 1) || (T > 1 && apart < K)) return py::none();
-    LaunchStream launch(device, given);
-    at::Tensor q = matrix(T, K, x, E4M3), scales = matrix(block_rows == 1 ? T : blocks(T), blocks(K), x, at::kFloat);
-    return outcome(g_quantize(x.data_ptr(), type, T > 1 ? apart : K, q.data_ptr(), (float*)scales.data_ptr(), (int)T, (int)K, (int)block_rows, launch.stream), q, scales);
+    at::Tensor q, scales;
+    int status;
+    {
+        py::gil_scoped_release unlocked;
+        LaunchStream launch(device, given);
+        q = matrix(T, K, x, E4M3);
+        scales = matrix(block_rows == 1 ? T : blocks(T), blocks(K), x, at::kFloat);
+        status = g_quantize(x.data_ptr(), type, T > 1 ? apart : K, q.data_ptr(), (float*)scales.data_ptr(), (int)T, (int)K, (int)block_rows, launch.stream);
+    }
+    return outcome(status, q, scales);
 }
 
 py::object add_rmsnorm(const at::Tensor& x, const std::optional<at::Tensor>& add, const at::Tensor& weight, double eps, int64_t parts, bool write_x,
@@ -90,10 +99,17 @@ py::object add_rmsnorm(const at::Tensor& x, const std::optional<at::Tensor>& add
     } else if (write_x && add) {
         keep = x.data_ptr();
     }
-    LaunchStream launch(device, given);
-    at::Tensor q = matrix(T, E, x, E4M3), scales = matrix(T, blocks(E), x, at::kFloat);
-    return outcome(g_norm((const float*)x.data_ptr(), add ? add->data_ptr() : nullptr, type, (int)parts, T * E, (const float*)weight.data_ptr(), (float)eps, nullptr, (int)T, (int)T,
-                          (int)E, (float*)keep, q.data_ptr(), (float*)scales.data_ptr(), launch.stream), q, scales);
+    at::Tensor q, scales;
+    int status;
+    {
+        py::gil_scoped_release unlocked;
+        LaunchStream launch(device, given);
+        q = matrix(T, E, x, E4M3);
+        scales = matrix(T, blocks(E), x, at::kFloat);
+        status = g_norm((const float*)x.data_ptr(), add ? add->data_ptr() : nullptr, type, (int)parts, T * E, (const float*)weight.data_ptr(), (float)eps, nullptr, (int)T, (int)T,
+                        (int)E, (float*)keep, q.data_ptr(), (float*)scales.data_ptr(), launch.stream);
+    }
+    return outcome(status, q, scales);
 }
 
 py::object gated(const at::Tensor& gate_up, int64_t parts, int64_t given) {
@@ -102,9 +118,16 @@ py::object gated(const at::Tensor& gate_up, int64_t parts, int64_t given) {
     const int64_t T = gate_up.size(-2), width = gate_up.size(-1), F = width / 2;
     const int device = gate_up.get_device(), type = code(gate_up);
     if (device != c10::cuda::current_device() || type < 0 || !size_ok(T) || !size_ok(width) || width % 2 || !gate_up.is_contiguous()) return py::none();
-    LaunchStream launch(device, given);
-    at::Tensor q = matrix(T, F, gate_up, E4M3), scales = matrix(T, blocks(F), gate_up, at::kFloat);
-    return outcome(g_gated(gate_up.data_ptr(), type, (int)parts, T * width, q.data_ptr(), (float*)scales.data_ptr(), (int)T, (int)F, nullptr, launch.stream), q, scales);
+    at::Tensor q, scales;
+    int status;
+    {
+        py::gil_scoped_release unlocked;
+        LaunchStream launch(device, given);
+        q = matrix(T, F, gate_up, E4M3);
+        scales = matrix(T, blocks(F), gate_up, at::kFloat);
+        status = g_gated(gate_up.data_ptr(), type, (int)parts, T * width, q.data_ptr(), (float*)scales.data_ptr(), (int)T, (int)F, nullptr, launch.stream);
+    }
+    return outcome(status, q, scales);
 }
 
 // The whole product, cut as the plan says; bf16: of the output.
@@ -117,11 +140,16 @@ py::object gemm(const at::Tensor& x, const at::Tensor& xs, const at::Tensor& w, 
         return py::none();
     int tile = 0, splits = 0;
     if (const int status = g_plan((int)M, (int)N, (int)K, 1, &tile, &splits)) return py::int_(status);
-    LaunchStream launch(device, given);
-    at::Tensor out = matrix(M, N, x, bf16 ? at::kBFloat16 : at::kFloat), parts;
-    if (splits > 1) parts = at::empty({splits, M, N}, x.options().dtype(at::kFloat));
-    const int status = g_gemm(x.data_ptr(), (const float*)xs.data_ptr(), w.data_ptr(), (const float*)ws.data_ptr(), out.data_ptr(), bf16 ? 1 : 0, (int)M, (int)N, (int)K, tile, splits,
-                              splits > 1 ? (float*)parts.data_ptr() : nullptr, early_w ? 1 : 0, nullptr, launch.stream);
+    at::Tensor out, parts;
+    int status;
+    {
+        py::gil_scoped_release unlocked;
+        LaunchStream launch(device, given);
+        out = matrix(M, N, x, bf16 ? at::kBFloat16 : at::kFloat);
+        if (splits > 1) parts = at::empty({splits, M, N}, x.options().dtype(at::kFloat));
+        status = g_gemm(x.data_ptr(), (const float*)xs.data_ptr(), w.data_ptr(), (const float*)ws.data_ptr(), out.data_ptr(), bf16 ? 1 : 0, (int)M, (int)N, (int)K, tile, splits,
+                        splits > 1 ? (float*)parts.data_ptr() : nullptr, early_w ? 1 : 0, nullptr, launch.stream);
+    }
     if (status != 0) return py::int_(status);
     return py::cast(out);
 }
