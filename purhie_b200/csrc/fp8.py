@@ -38,7 +38,7 @@ register_signatures("fp8", {
 BLOCK = 128
 E4M3, F32 = torch.float8_e4m3fn, torch.float32
 MAX_NORM_WIDTH = 32768
-_LIMIT = 2 ** 31 - 1
+_LIMIT = 2 ** 31 - 1                 # of every count: the launchers take 32-bit numbers, and ctypes cuts what is longer
 ERRORS = {131: "the copies waited too long for a free stage", 132: "the products waited too long", 133: "the epilogue waited too long for an accumulator"}
 
 
@@ -159,14 +159,14 @@ def add_rmsnorm(x: torch.Tensor, add: Optional[torch.Tensor], weight: torch.Tens
         raise KernelError("add_rmsnorm: x must be contiguous float32")
     if weight.dtype != torch.float32 or weight.shape != (E,) or not weight.is_contiguous():
         raise KernelError(f"add_rmsnorm: weight must be contiguous float32 [{E}]")
-    if add is not None and (add_splits < 1 or add.shape != ((T, E) if add_splits == 1 and add.dim() == 2 else (add_splits, T, E)) or not add.is_contiguous()):
+    if add is not None and (not 1 <= add_splits <= _LIMIT or add.shape != ((T, E) if add_splits == 1 and add.dim() == 2 else (add_splits, T, E)) or not add.is_contiguous()):
         raise KernelError(f"add_rmsnorm: add must be contiguous {add_splits} x [{T}, {E}], got {tuple(add.shape)}")
     if not eps >= 0.0:
         raise KernelError(f"add_rmsnorm: eps must not be negative, got {eps}")
     n = T
     if rows is not None:
-        if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous() or x_out is not None:
-            raise KernelError("add_rmsnorm: rows must be a contiguous int32 vector, and x_out does not go with it")
+        if rows.dtype != torch.int32 or rows.dim() != 1 or rows.shape[0] > _LIMIT or not rows.is_contiguous() or x_out is not None:
+            raise KernelError(f"add_rmsnorm: rows must be a contiguous int32 vector of at most {_LIMIT}, and x_out does not go with it")
         n = rows.shape[0]
     if n and not T:
         raise KernelError("add_rmsnorm: there are no rows to pick from")
@@ -209,8 +209,8 @@ def gated(gate_up: torch.Tensor, out: Optional[torch.Tensor] = None, scales: Opt
         if got is not None:
             return _made(got)
     shape = gate_up.shape
-    if len(shape) != (2 if splits == 1 else 3) or shape[-1] % 2 or not 0 < shape[-1] <= _LIMIT or splits < 1 or (splits > 1 and shape[0] != splits) or \
-            not gate_up.is_contiguous():
+    if len(shape) != (2 if splits == 1 else 3) or shape[-1] % 2 or not 0 < shape[-1] <= _LIMIT or shape[-2] > _LIMIT or not 1 <= splits <= _LIMIT or \
+            (splits > 1 and shape[0] != splits) or not gate_up.is_contiguous():
         raise KernelError(f"gated: gate_up must be contiguous (gate, up) pairs in {splits} parts, got {tuple(shape)}")
     T, F = shape[-2], shape[-1] // 2
     code = ops._code(gate_up.dtype)
