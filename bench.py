@@ -52,6 +52,11 @@ def peaks():
     return dict(FALLBACK_PEAKS, source="fallback")
 
 
+def prefill_fraction(matrix_flops, other_flops, ms, bf16_tflops, eight_bit):
+    """A prefill's floor over its time: all of it at the bf16 rate, or, with the layers' matrices in 8 bits, those at twice that."""
+    return (matrix_flops / (2.0 if eight_bit else 1.0) + other_flops) / (ms * 1e-3) / 1e12 / bf16_tflops
+
+
 class ClockSampler:
     """Samples SM clocks and throttle reasons with nvidia-smi while the timed region runs."""
     FIELDS = ("clocks.sm,clocks.max.sm,clocks_event_reasons.hw_slowdown,clocks_event_reasons.hw_thermal_slowdown,"
@@ -362,11 +367,15 @@ def main():
     T, E, FF, V = PREFILL_TOKENS, cfg.hidden_size, cfg.intermediate_size, cfg.vocab_size
     qw, kvw, D = cfg.q_width, cfg.kv_width, cfg.head_dim
     layer_mm = E * (qw + 2 * kvw) + qw * E + 3 * E * FF
-    prefill_flops = cfg.num_hidden_layers * (2.0 * T * layer_mm + 4.0 * cfg.num_attention_heads * D * T * (T + 1) / 2) + 2.0 * V * E
-    tflops = prefill_flops / (prefill_ms * 1e-3) / 1e12
+    matrix_flops = cfg.num_hidden_layers * 2.0 * T * layer_mm
+    other_flops = cfg.num_hidden_layers * 4.0 * cfg.num_attention_heads * D * T * (T + 1) / 2 + 2.0 * V * E
+    tflops = (matrix_flops + other_flops) / (prefill_ms * 1e-3) / 1e12
+    fraction = lambda peak: round(prefill_fraction(matrix_flops, other_flops, prefill_ms, peak, args.gemm == "fp8"), 4)
     prefill = {"value": round(T / prefill_ms * 1e3, 1), "tokens": T, "ms": round(prefill_ms, 3),
-               "frac": round(tflops / pk["bf16_tflops"], 4), "frac_of_sustained": round(tflops / pk["bf16_tflops_sustained"], 4),
+               "frac": fraction(pk["bf16_tflops"]), "frac_of_sustained": fraction(pk["bf16_tflops_sustained"]),
                "tflops": round(tflops, 1), "peak": pk["source"]}
+    if args.gemm == "fp8":
+        prefill["frac_peak"] = "the layers' matrices at twice the bf16 rate, attention and the output matrix at the bf16 rate"
 
     # ---- prefixes of 2,048 tokens for every request ---------------------------------------------------
     for i in range(max_batch):
