@@ -86,6 +86,15 @@ void rows_context(PartProbe& p, int T, StepContext& ctx) {
     ctx.decode_only = false;
     fill_context(p, ctx);
 }
+// The rows x in 8 bits, as a norm in front gives them: bytes, with their scales in ctx.row8_scales.
+Tensor in_eight_bits(PartProbe& p, const Tensor& x, StepContext& ctx) {
+    const int64_t T = x.shape[0], E = x.shape[1];
+    Tensor q = p.ws.get("probe_x8", {T, E}, DType::U8), scales = p.ws.get("probe_x8_scales", {T, (E + 127) / 128}, DType::F32);
+    const Fp8Kernels& k = fp8_kernels();
+    QE_LAUNCH(k, k.quantize(x.data, x.code(), E, q.data, scales.as<float>(), (int)T, (int)E, 1, p.stream));
+    ctx.row8_scales = scales.as<float>();
+    return q;
+}
 #define PROBE(h) (*static_cast<PartProbe*>(h))
 }  // namespace
 
@@ -208,6 +217,28 @@ API int qe_part_norm(void* h, const float* x, const float* add, int T, int E, fl
     });
 }
 
+// The same norm over all rows in 8 bits (Norm::forward_eight_bit): `add` (optional) is the pending addend in `splits` parts, rounded to
+// bfloat16 where asked for; out_q [T, E] e4m3, out_scales [T, ceil(E / 128)].
+API int qe_part_norm_eight_bit(void* h, const float* x, const float* add, int splits, int add_bf16, int T, int E, float* out_x, uint8_t* out_q, float* out_scales) {
+    return guarded([&] {
+        PartProbe& p = PROBE(h);
+        auto* norm = dynamic_cast<Norm*>(p.part.get());
+        if (!norm) throw Error(kInvalidArg, "not a norm");
+        StepContext ctx;
+        rows_context(p, T, ctx);
+        ResidualStream stream;
+        stream.x = upload(p, "probe_x", x, {T, E}, DType::F32);
+        if (add) stream.add(Addend(upload(p, "probe_add", add, {splits, T, E}, add_bf16 ? DType::BF16 : DType::F32), splits));
+        Tensor y = norm->forward_eight_bit(stream, ctx);
+        if (!y.defined() || !ctx.row8_scales) throw Error(kInvalidState, "the norm has no form in 8 bits");
+        if (stream.has_pending) throw Error(kInvalidState, "the norm left the pending addend in the stream");
+        download(p, stream.x, 1, out_x);
+        QE_CUDA(cudaMemcpy(out_q, y.data, (size_t)T * E, cudaMemcpyDeviceToHost));
+        QE_CUDA(cudaMemcpy(out_scales, ctx.row8_scales, (size_t)T * ((E + 127) / 128) * 4, cudaMemcpyDeviceToHost));
+        return 0;
+    });
+}
+
 // Position encoding: n_rot, pairing, column and the rotation table's shape; the table itself with qe_part_position_table.
 API const char* qe_part_position_info(void* h) {
     return guarded_text([&] {
@@ -267,8 +298,9 @@ API int qe_part_head(void* h, const float* xn, int T, int E, float* out) {
     });
 }
 
-// Feed-forward: x [T, E] (rounded to the compute dtype) -> the addend, partial sums added up, as float32 [T, E].
-API int qe_part_feed_forward(void* h, const float* x, int T, int E, float* out) {
+// Feed-forward: x [T, E] (rounded to the compute dtype; in 8 bits where asked for and the part takes them) -> the addend, partial sums
+// added up, as float32 [T, E].
+static int run_feed_forward(void* h, const float* x, int T, int E, bool eight_bit, float* out) {
     return guarded([&] {
         PartProbe& p = PROBE(h);
         auto* ff = dynamic_cast<FeedForward*>(p.part.get());
@@ -276,13 +308,16 @@ API int qe_part_feed_forward(void* h, const float* x, int T, int E, float* out) 
         StepContext ctx;
         rows_context(p, T, ctx);
         Tensor xin = upload(p, "probe_x", x, {T, E}, p.dtype);
-        Addend y = ff->forward(xin, ctx);
+        if (eight_bit && !ff->takes_eight_bit_rows(ctx)) throw Error(kInvalidState, "the part takes no rows in 8 bits");
+        Addend y = ff->forward(eight_bit ? in_eight_bits(p, xin, ctx) : xin, ctx);
         if (!y.tensor.defined()) throw Error(kInvalidState, "the part added into a residual that was not there");
         download(p, y.tensor, y.splits, out);
         check_errors(p);
         return 0;
     });
 }
+API int qe_part_feed_forward(void* h, const float* x, int T, int E, float* out) { return run_feed_forward(h, x, T, E, false, out); }
+API int qe_part_feed_forward_eight_bit(void* h, const float* x, int T, int E, float* out) { return run_feed_forward(h, x, T, E, true, out); }
 
 // Mixer: a cache of its own first, then steps.
 API int qe_part_mixer_cache(void* h, int page_size, int num_pages, int max_requests, int poison) {
@@ -299,8 +334,9 @@ API int qe_part_mixer_cache(void* h, int page_size, int num_pages, int max_reque
 API int qe_part_mixer_add_request(void* h, long long id) { return guarded([&] { PROBE(h).cache->add_request(id); return 0; }); }
 API int qe_part_mixer_release(void* h, long long id) { return guarded([&] { PROBE(h).cache->release(id); return 0; }); }
 // One step: segment s brings n_new[s] new rows of request requests[s]; x holds all rows [T, E] in segment order.
-// out: the mixer's addend, partial sums added up, float32 [T, E].
-API int qe_part_mixer_step(void* h, const long long* requests, const int* n_new, int n_segments, const float* x, int E, float* out) {
+// out: the mixer's addend, partial sums added up, float32 [T, E].  eight_bit: x comes in 8 bits.  reads_only: out is what a second layer of the
+// same weights gives that only reads the cache which the first has written.
+static int run_mixer_step(void* h, const long long* requests, const int* n_new, int n_segments, const float* x, int E, bool eight_bit, bool reads_only, float* out) {
     return guarded([&] {
         PartProbe& p = PROBE(h);
         auto* mixer = dynamic_cast<Mixer*>(p.part.get());
@@ -331,8 +367,14 @@ API int qe_part_mixer_step(void* h, const long long* requests, const int* n_new,
             context_from_layout(lay, *p.cache, 1, meta.as<int32_t>(), ctx, &want);
             fill_context(p, ctx);
             Tensor xin = upload(p, "probe_x", x, {T, E}, p.dtype);
+            if (eight_bit && !mixer->takes_eight_bit_rows(ctx)) throw Error(kInvalidState, "the part takes no rows in 8 bits");
+            if (eight_bit) xin = in_eight_bits(p, xin, ctx);
             CacheView view = p.cache->view(0, 0);
             Addend y = mixer->forward(xin, ctx, view);
+            if (reads_only) {
+                view.writable = false;
+                y = mixer->forward(xin, ctx, view);
+            }
             if (!y.tensor.defined()) throw Error(kInvalidState, "the part added into a residual that was not there");
             download(p, y.tensor, y.splits, out);
             check_errors(p);
@@ -343,4 +385,10 @@ API int qe_part_mixer_step(void* h, const long long* requests, const int* n_new,
         for (const StepEntry& e : entries) p.cache->advance(e.request, e.n_tokens);
         return 0;
     });
+}
+API int qe_part_mixer_step(void* h, const long long* requests, const int* n_new, int n_segments, const float* x, int E, float* out) {
+    return run_mixer_step(h, requests, n_new, n_segments, x, E, false, false, out);
+}
+API int qe_part_mixer_step_as(void* h, const long long* requests, const int* n_new, int n_segments, const float* x, int E, int eight_bit, int reads_only, float* out) {
+    return run_mixer_step(h, requests, n_new, n_segments, x, E, eight_bit != 0, reads_only != 0, out);
 }

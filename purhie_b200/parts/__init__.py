@@ -58,6 +58,9 @@ def _lib():
             ("qe_part_mixer_cache", c_int, [P, c_int, c_int, c_int, c_int]), ("qe_part_mixer_add_request", c_int, [P, c_longlong]),
             ("qe_part_mixer_release", c_int, [P, c_longlong]),
             ("qe_part_mixer_step", c_int, [P, POINTER(c_longlong), POINTER(c_int), c_int, F, c_int, F]),
+            ("qe_part_mixer_step_as", c_int, [P, POINTER(c_longlong), POINTER(c_int), c_int, F, c_int, c_int, c_int, F]),
+            ("qe_part_feed_forward_eight_bit", c_int, [P, F, c_int, c_int, F]),
+            ("qe_part_norm_eight_bit", c_int, [P, F, F, c_int, c_int, c_int, c_int, F, c_void_p, F]),
         ]:
             native.declare(name, res, args)
         _DECLARED = True
@@ -118,6 +121,16 @@ class PartProbe:
         native.check(_lib().qe_part_norm(self._h, _ptr(x), _ptr(add), T, E, _ptr(out_x), _ptr(out_y)))
         return out_x, out_y
 
+    def norm_eight_bit(self, x, add=None, add_dtype: str = "float32"):
+        """(the stream afterwards = x + the parts of ``add`` [parts, T, E], the normed rows' e4m3 bytes, their scales)."""
+        x = _f32(x)
+        add = None if add is None else _f32(add)
+        T, E = x.shape
+        out_x, q, scales = np.empty_like(x), np.empty((T, E), dtype=np.uint8), np.empty((T, -(-E // 128)), dtype=np.float32)
+        native.check(_lib().qe_part_norm_eight_bit(self._h, _ptr(x), _ptr(add), 1 if add is None else add.shape[0], int(add_dtype == "bfloat16"), T, E, _ptr(out_x),
+                                                   q.ctypes.data, _ptr(scales)))
+        return out_x, q, scales
+
     def position_info(self) -> Dict:
         return native.answer(_lib().qe_part_position_info(self._h))
 
@@ -139,10 +152,12 @@ class PartProbe:
         native.check(_lib().qe_part_head(self._h, _ptr(xn), xn.shape[0], xn.shape[1], _ptr(out)))
         return out
 
-    def feed_forward(self, x) -> np.ndarray:
+    def feed_forward(self, x, eight_bit: bool = False) -> np.ndarray:
+        """``eight_bit``: the part is handed its rows in 8 bits."""
         x = _f32(x)
         out = np.empty_like(x)
-        native.check(_lib().qe_part_feed_forward(self._h, _ptr(x), x.shape[0], x.shape[1], _ptr(out)))
+        run = _lib().qe_part_feed_forward_eight_bit if eight_bit else _lib().qe_part_feed_forward
+        native.check(run(self._h, _ptr(x), x.shape[0], x.shape[1], _ptr(out)))
         return out
 
     # ---- a mixer and its cache
@@ -155,15 +170,16 @@ class PartProbe:
     def release(self, request: int) -> None:
         native.check(_lib().qe_part_mixer_release(self._h, request))
 
-    def mixer_step(self, segments, x) -> np.ndarray:
+    def mixer_step(self, segments, x, eight_bit: bool = False, reads_only: bool = False) -> np.ndarray:
         """One step: ``segments`` = [(request, new rows)], ``x`` all rows [T, E] in segment order; the mixer's output
-        rows [T, E]."""
+        rows [T, E].  ``eight_bit``: the mixer is handed its rows in 8 bits.  ``reads_only``: the output of a second layer of the
+        same weights, which reads the cache that the first one has written."""
         x = _f32(x)
         n = len(segments)
         reqs = (c_longlong * n)(*[s[0] for s in segments])
         rows = (c_int * n)(*[s[1] for s in segments])
         out = np.empty_like(x)
-        native.check(_lib().qe_part_mixer_step(self._h, reqs, rows, n, _ptr(x), x.shape[1], _ptr(out)))
+        native.check(_lib().qe_part_mixer_step_as(self._h, reqs, rows, n, _ptr(x), x.shape[1], int(eight_bit), int(reads_only), _ptr(out)))
         return out
 
 
