@@ -314,6 +314,9 @@ def main():
         print(f"bench.py: this engine runs on one GPU; --gpus {args.gpus} is not supported")
         return 2
     args.warmup = max(args.warmup, 3)
+    if args.design and args.gemm != "auto":
+        print("bench.py: --design measures its models in bfloat16; --gemm does not go with it")
+        return 2
     if args.design:
         return design_bench(args)
 
