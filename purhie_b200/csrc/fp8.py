@@ -66,14 +66,9 @@ def _stream(what: str, first: torch.Tensor, *others) -> int:
 _calls = None
 
 
-def _step(first: torch.Tensor):
-    """The compiled step for a plain call on `first`, or None where there is nothing for it to do: a tensor that is not on a device
-    is refused by the face's own checks, without compiling anything."""
-    return (_calls or _load_calls()) if first.is_cuda else None
-
-
 def _load_calls():
-    """The extension that makes a plain call in one step (fp8_calls.cpp), with the launchers it needs."""
+    """The extension that makes a plain call in one step (fp8_calls.cpp), with the launchers it needs.  Host tensors are refused by the
+    faces' own checks, without compiling it."""
     global _calls
     calls = load_extension("fp8_calls")
     calls.set_launchers(*(ctypes.cast(ops._fn("fp8", f"ph_{n}")[0], c_void_p).value
@@ -119,8 +114,8 @@ def quantize(x: torch.Tensor, out: Optional[torch.Tensor] = None, scales: Option
     """x [T, K] (float32 or bfloat16, its rows ``x.stride(0)`` apart) in 8 bits: out [T, K] and scales [ceil(T / block_rows),
     ceil(K / 128)].  ``block_rows``: 1 for the rows of a product, 128 for a weight."""
     if out is None and scales is None:
-        step = _step(x)
-        got = step and step.quantize(x, block_rows, _scope())
+        calls = _calls or (x.is_cuda and _load_calls())
+        got = calls.quantize(x, block_rows, _scope()) if calls else None
         if got is not None:
             return _made(got)
     T, K = _matrix("quantize", "x", x)
@@ -148,8 +143,8 @@ def add_rmsnorm(x: torch.Tensor, add: Optional[torch.Tensor], weight: torch.Tens
     false or there is nothing to add).  ``rows`` (int32 [n]) picks the rows that are normed, in that order (out [n, E]); nothing is
     kept then, and a number outside 0 .. T - 1 leaves its row of out and scales as it was."""
     if out is None and scales is None and rows is None:
-        step = _step(x)
-        got = step and step.add_rmsnorm(x, add, weight, eps, add_splits, write_x, x_out, _scope())
+        calls = _calls or (x.is_cuda and _load_calls())
+        got = calls.add_rmsnorm(x, add, weight, eps, add_splits, write_x, x_out, _scope()) if calls else None
         if got is not None:
             return _made(got)
     T, E = _matrix("add_rmsnorm", "x", x)
@@ -204,8 +199,8 @@ def gated(gate_up: torch.Tensor, out: Optional[torch.Tensor] = None, scales: Opt
     with ``splits`` > 1 (float32 or bfloat16), to out [T, F], scales [T, ceil(F / 128)].  ``gate``: None (silu), (alpha, limit,
     shift) of the clamped swish, or "gelu_tanh"."""
     if out is None and scales is None and gate is None:
-        step = _step(gate_up)
-        got = step and step.gated(gate_up, splits, _scope())
+        calls = _calls or (gate_up.is_cuda and _load_calls())
+        got = calls.gated(gate_up, splits, _scope()) if calls else None
         if got is not None:
             return _made(got)
     shape = gate_up.shape
@@ -249,8 +244,8 @@ def gemm(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: tor
     kernel that may still run when the product starts (a model's weight), so its first tiles may be read before the kernel in
     front has ended."""
     if out is None and not tile and not splits and (out_dtype is torch.bfloat16 or out_dtype is F32):
-        step = _step(x)
-        got = step and step.gemm(x, x_scales, w, w_scales, out_dtype is torch.bfloat16, early_w, _scope())
+        calls = _calls or (x.is_cuda and _load_calls())
+        got = calls.gemm(x, x_scales, w, w_scales, out_dtype is torch.bfloat16, early_w, _scope()) if calls else None
         if got is not None:
             return _made(got)
     M, K = _matrix("gemm_fp8", "x", x)
