@@ -70,8 +70,10 @@ inference_model_t* inference_load_model(const char* model_dir);
  * options_json: NULL or {"gemm": "auto|tcgen05|simple|fp8", "attention": "auto|flash|generic"}.  "fp8" (bfloat16 models): the
  * matrices of the attention parts and of the feed-forwards that are not routed are brought to 8 bits when they are loaded
  * (e4m3, a scale for each block of 128 x 128), their rows in every step (a scale for each 128 values), and multiplied that way;
- * the embedding, the output matrix and every other part stay as they are.  Half the memory and twice the decode rate of the
- * matrices concerned, at 8 bits' precision. */
+ * the embedding, the output matrix, a matrix stored in float32 and every other part stay as they are.  Weights are read in 16 or 32
+ * bits only.  Half the memory of the matrices concerned; on a B200 the 8B shape decodes 1.2 (64 rows) to 1.33 (1 and 8 rows)
+ * times as fast as in bfloat16 and reads a prompt of 2,048 tokens 1.16 times as fast.  The precision is that of 8 bits; a
+ * feed-forward's gate and up sums are besides rounded to bfloat16 in front of the activation where a step has few rows. */
 inference_model_t* inference_load_model_ex(const char* model_dir, const char* dtype, const char* options_json);
 /* Seeded random weights made on the device for the configuration in config_json (the text of a config.json):
  * matrices N(0, 0.02), norm weights 1.  The values are those inference_write_random_model stores. */

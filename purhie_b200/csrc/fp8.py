@@ -287,7 +287,7 @@ def gemm_gated(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
                scales: Optional[torch.Tensor] = None, *, gate=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """What ``gated`` makes of ``gemm``'s float32 product, without the product going to memory: w [N, K] holds the rows of gate and up in
     turn (N a multiple of 256, K of 16), out [M, N / 2], scales [M, N / 256]; ``gate`` as in ``gated``.  For many tokens: it runs on
-    pairs of CTAs with K whole, whatever M is."""
+    pairs of CTAs with K whole, whatever M is.  Where ``plan`` gives anything but (256, 1), ``gemm`` and ``gated`` can be faster."""
     M, K = _matrix("gemm_gated", "x", x)
     N, K2 = _matrix("gemm_gated", "w", w)
     if x.dtype is not E4M3 or w.dtype is not E4M3 or not x.is_contiguous() or not w.is_contiguous():

@@ -463,9 +463,9 @@ __device__ __forceinline__ void store_gated(const Params& p, float* acc, float* 
 
 // GATED: the epilogue applies the gated activation and brings its values to 8 bits.  A tile's 256 features are 128 (gate, up) pairs, one
 // block of the result for each of its rows: the two warps that hold a row's halves tell each other their largest magnitudes.  The tensor
-// cores stand still while a tile's 64 exponentials a thread are made (2048 x 24576 x 4096: 244 us, 217 and 25 as two kernels; 8192 rows
-// 876, 825 and 97), but the product's 100 MB neither leave nor come back: a prompt of 2,048 tokens through 36 such layers, at the power
-// limit, takes 22.7 ms for 23.25.
+// cores stand still while a tile's 64 exponentials a thread are made, but the product's 100 MB neither leave nor come back: in a graph, over
+// weights that L2 does not hold, 512 x 24576 x 4096 takes 73 us and 75 as two kernels, 2,048 rows 252 and 258, 8,192 rows 915 and 942; a
+// prompt of 2,048 tokens through 36 such layers, at the power limit, 22.7 ms for 23.25.
 template <bool GATED>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_out, Params p) {

@@ -76,6 +76,9 @@ public:
                 return down_(act8, ctx, "ff_out", DType::F32, T, true, false, ctx.residual, nullptr, &ctx.norm_ahead);
             }
         }
+        // (Sums that nobody has to add up come in the compute dtype.  With the activation in this product's epilogue they stay float32 in front
+        // of it; where a kernel behind it applies the activation, as with 8-bit matrices and K whole at few rows, they are rounded to
+        // bfloat16 first: off by up to 2^-8, in front of a rounding to 8 bits of up to 2^-4.)
         Addend gu = gate_up_(x, ctx, "gate_up", compute_dtype, T, true, true, nullptr, &ctx.row_scale, nullptr,
                              gate_.kind ? gate_constants : nullptr);
         Tensor act;

@@ -158,6 +158,10 @@ Tensor Linear::gated_eight_bit(const Tensor& x, StepContext& ctx, const std::str
     const Fp8Kernels& k = fp8_kernels();
     int tile = 0, splits = 0;
     if (k.plan(M, N, K, 0, &tile, &splits) != 0) throw KernelError(k.last_error());
+    // Where the plain product would go to that kernel, K whole, the two in one are at most 1 % slower than one behind the other and mostly
+    // faster (160 to 8,192 rows of 6144 x 1024, 24576 x 4096 and 51200 x 5120, in graphs: 320 rows of 24576 x 4096 72.6 us for
+    // 72.3, 2,048 rows 252 for 258, 8,192 rows of 6144 x 1024 90 for 103); where it would go to smaller tiles, up to 37 % slower
+    // (160 rows of 6144 x 1024 11.9 us for 8.7).
     if (tile != kPairTile || splits != 1) return Tensor();
     const float* row_scales = nullptr;
     const void* q = eight_bit_rows(x, ctx, M, &row_scales);
